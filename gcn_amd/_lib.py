@@ -22,6 +22,7 @@ ERR_HIP = -4
 ERR_UNSUPPORTED = -5
 ERR_COMM = -6
 COMM_ID_BYTES = 128
+F32, BF16, F16 = 0, 1, 2               # gcnx_dtype
 
 
 class GcnxError(RuntimeError):
@@ -49,9 +50,20 @@ class CsrStruct(C.Structure):
                 ("spmm_chunk", C.c_int32), ("gather_keep", C.c_void_p)]
 
 
+class AttentionStruct(C.Structure):
+    """Mirror of ``struct gcnx_attention``."""
+    _fields_ = [("a", C.POINTER(CsrStruct)), ("use_values", C.c_int32), ("dtype", C.c_int32),
+                ("edge_mask", C.c_void_p), ("mask_index", C.c_void_p), ("max_row_nnz", C.c_int64),
+                ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float),
+                ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),
+                ("k", C.c_void_p), ("k_row", C.c_int64), ("k_head", C.c_int64),
+                ("v", C.c_void_p), ("v_row", C.c_int64), ("v_head", C.c_int64)]
+
+
 _i32, _i64, _u64, _f32, _f64 = C.c_int32, C.c_int64, C.c_uint64, C.c_float, C.c_double
 _p, _sz, _int = C.c_void_p, C.c_size_t, C.c_int
 _csr_p = C.POINTER(CsrStruct)
+_att_p = C.POINTER(AttentionStruct)
 
 # name -> (restype, argtypes); must list every function include/gcnx.h declares.
 SIGNATURES = {
@@ -119,6 +131,11 @@ SIGNATURES = {
     "gcnx_gemm_workspace_bytes": (_sz, [_int, _int, _i64, _i64, _i64]),
     "gcnx_gemm_f32": (_int, [_int, _int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _f32, _f32,
                              _int, _p, _sz, _p]),
+    "gcnx_attention_workspace_bytes": (_sz, [_att_p]),
+    "gcnx_attention_forward": (_int, [_att_p, _p, _p, _i64, _i64, _p, _p, _sz, _p]),
+    "gcnx_attention_backward_workspace_bytes": (_sz, [_att_p, _i64]),
+    "gcnx_attention_backward": (_int, [_att_p, _p, _csr_p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p,
+                                       _p, _p, _sz, _p]),
     "gcnx_xent_workspace_bytes": (_sz, [_i64]),
     "gcnx_masked_softmax_xent_f32": (_int, [_i64, _i32, _p, _i64, _p, _i64, _p, _f64, _p, _p, _i64,
                                             _p, _sz, _p]),

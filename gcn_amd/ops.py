@@ -465,6 +465,141 @@ def gemm_autograd(a, b, relu=False):
     return _GemmFn.apply(a, b, relu)
 
 
+# ------------------------------------------------------------------- attention
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _check_heads(t, name, rows, dim=None, like=None):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise RuntimeError("%s must be a CUDA (ROCm) tensor; gcn_amd has no CPU path" % name)
+    if t.dtype not in _DTYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError("%s must be [rows, heads, head_dim] with contiguous head vectors" % name)
+    if t.shape[0] != rows:
+        raise ValueError("%s has %d rows, the matrix asks for %d" % (name, t.shape[0], rows))
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError("%s differs in dtype or device" % name)
+    if dim is not None and t.shape[2] != dim:
+        raise ValueError("%s has head_dim %d, expected %d" % (name, t.shape[2], dim))
+
+
+def _attention_struct(a, q, k, v, scale, use_values, mask):
+    _check_heads(q, "q", a.n_rows)
+    _check_heads(k, "k", a.n_cols, q.shape[2], q)
+    _check_heads(v, "v", a.n_cols, q.shape[2], q)
+    if q.device != a.device:
+        raise ValueError("the matrix and q live on different devices")
+    heads, kv, dim = q.shape[1], k.shape[1], q.shape[2]
+    if v.shape[1] != kv or kv < 1 or heads < 1 or heads % kv:
+        raise ValueError("%d query heads cannot share %d key and %d value heads" % (heads, kv, v.shape[1]))
+    if not 1 <= dim <= 256:
+        raise ValueError("head_dim must be 1..256, got %d" % dim)
+    midx = None
+    if mask is not None:
+        if mask.dtype != torch.uint8 or mask.dim() != 1 or mask.numel() != a.nnz or not mask.is_contiguous() or \
+                mask.device != a.device:
+            raise ValueError("mask must be contiguous uint8 with one byte per nonzero on A's device")
+        midx = a.input_index
+    return _lib.AttentionStruct(
+        C.pointer(a._struct), int(bool(use_values)), _DTYPES[q.dtype], mask.data_ptr() if mask is not None else None,
+        midx.data_ptr() if midx is not None else None, a.max_row_nnz(), heads, kv, dim,
+        float(scale) if scale is not None else dim ** -0.5, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+        k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1))
+
+
+def _scratch(nbytes, device):
+    # from torch's allocator, which orders the memory by stream and owns it in a
+    # capture: two streams, or two recorded graphs, never share it
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, want_stats=False):
+    """Softmax attention of every row of ``a`` (a :class:`Csr`) over its columns:
+    ``out[i, h] = sum_j softmax_j(scale * <q[i, h], k[j, h']> + a[i, j]) * v[j, h']``
+    with the matrix values as logit shifts only if ``use_values``; query head ``h``
+    reads key head ``h' = h // (heads / kv_heads)``.  ``q`` [n_rows, heads, head_dim],
+    ``k`` and ``v`` [n_cols, kv_heads, head_dim], float32, bfloat16 or float16, any
+    strides between head vectors; ``scale`` defaults to ``head_dim ** -0.5``.
+    ``mask`` (uint8, in the order of the tuple ``A`` was built from) takes the
+    edges with 0 out of the softmax, as a value of -inf does; a row with no edge
+    left gives zeros.  With ``want_stats`` returns ``(out, stats)``, what
+    :func:`attention_bwd` needs.  The attention-weighted sibling of :func:`spmm`
+    (reference gcn/layers.py:219 sums the neighbours with fixed weights)."""
+    lib = _lib.load()
+    p = _attention_struct(a, q, k, v, scale, use_values, mask)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_heads(out, "out", a.n_rows, q.shape[2], q)
+        if out.shape[1] != q.shape[1] or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+            raise ValueError("out must be [n_rows, heads, head_dim] of distinct elements")
+    stats = torch.empty((a.n_rows, q.shape[1], 2), dtype=torch.float32, device=q.device) if want_stats else None
+    with torch.cuda.device(q.device):
+        ws = _scratch(lib.gcnx_attention_workspace_bytes(C.byref(p)), q.device)
+        _lib.check(lib.gcnx_attention_forward(C.byref(p), _ptr(a.chunk_row), _ptr(out), out.stride(0), out.stride(1),
+                                              _ptr(stats), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+    return (out, stats) if want_stats else out
+
+
+def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, mask=None, need_q=True, need_kv=True):
+    """``(dq, dk, dv)`` of :func:`attention` for the gradient ``d_out`` of its output,
+    from its ``out`` and ``stats`` (the probabilities are formed again, edge by
+    edge).  The gradients of shared key heads are summed over the query heads that
+    share them.  ``need_q`` / ``need_kv`` False leaves those gradients out (None).
+    Uses the transpose of ``a`` (built at its first use)."""
+    lib = _lib.load()
+    p = _attention_struct(a, q, k, v, scale, use_values, mask)
+    for t, name in ((out, "out"), (d_out, "d_out")):
+        _check_heads(t, name, a.n_rows, q.shape[2], q)
+        if t.shape[1] != q.shape[1]:
+            raise ValueError("%s has %d heads, expected %d" % (name, t.shape[1], q.shape[1]))
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (a.n_rows, q.shape[1], 2) or not stats.is_contiguous() or \
+            stats.device != q.device:
+        raise ValueError("stats must be what attention(..., want_stats=True) returned")
+    if not need_q and not need_kv:
+        return None, None, None
+    at = a.transpose()
+    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    dq = new(q) if need_q else None
+    dk, dv = (new(k), new(v)) if need_kv else (None, None)
+    midx = at.input_index if mask is not None else None
+    with torch.cuda.device(q.device):
+        ws = _scratch(lib.gcnx_attention_backward_workspace_bytes(C.byref(p), at.max_row_nnz()), q.device)
+        _lib.check(lib.gcnx_attention_backward(
+            C.byref(p), _ptr(a.chunk_row), at.struct_ref(), _ptr(at.chunk_row), _ptr(midx), at.max_row_nnz(), _ptr(out),
+            out.stride(0), out.stride(1), _ptr(stats), _ptr(d_out), d_out.stride(0), d_out.stride(1), _ptr(dq), _ptr(dk),
+            _ptr(dv), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+    return dq, dk, dv
+
+
+class _AttentionFn(torch.autograd.Function):
+    """Gradients w.r.t. q, k, v; none reaches the matrix values or the mask."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, a, scale, use_values, mask):
+        out, stats = attention(a, q, k, v, scale, use_values, mask, want_stats=True)
+        ctx.save_for_backward(q, k, v, out, stats)
+        ctx.how = (a, scale, use_values, mask)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        q, k, v, out, stats = ctx.saved_tensors
+        a, scale, use_values, mask = ctx.how
+        if d_out.stride(2) != 1 and d_out.shape[2] > 1:
+            d_out = d_out.contiguous()
+        dq, dk, dv = attention_bwd(a, q, k, v, out, stats, d_out, scale, use_values, mask, ctx.needs_input_grad[0],
+                                   ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None, None
+
+
+def attention_autograd(a, q, k, v, scale=None, use_values=False, mask=None):
+    """:func:`attention` on the autograd tape."""
+    return _AttentionFn.apply(q, k, v, a, scale, use_values, mask)
+
+
 # ------------------------------------------------------------- loss / accuracy
 def masked_softmax_xent(logits, labels, mask, want_grad=True, mask_total=0.0, grad_out=None):
     """Returns ``(loss_acc, grad)``: ``loss_acc`` is a 2-element device tensor

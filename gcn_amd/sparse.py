@@ -80,6 +80,7 @@ class Csr(object):
         self.input_index = input_index
         self.device = row_ptr.device
         self._t = None
+        self._max_row = None
         self.gather_keep = None
         self._struct = _lib.CsrStruct(self.n_rows, self.n_cols, self.nnz,
                                       row_ptr.data_ptr(), col_idx.data_ptr(), val.data_ptr(),
@@ -104,6 +105,15 @@ class Csr(object):
     @spmm_chunk.setter
     def spmm_chunk(self, value):
         self._struct.spmm_chunk = int(value)
+
+    def max_row_nnz(self):
+        """The most nonzeros of a row, looked up once (a host synchronisation) and
+        kept; 0 = unknown while a stream capture forbids the look-up."""
+        if self._max_row is None:
+            if torch.cuda.is_current_stream_capturing():
+                return 0
+            self._max_row = int((self.row_ptr[1:] - self.row_ptr[:-1]).max().item()) if self.n_rows else 0
+        return self._max_row
 
     # -------------------------------------------------------------- cache hint
     def column_degrees(self):

@@ -513,6 +513,62 @@ int gcnx_gemm_dropout_at_rows_f32(int64_t M, int64_t N, int64_t K, const float *
                                   const float *B, int64_t ldb, float *C, int64_t ldc, float alpha,
                                   float beta, void *ws, size_t ws_bytes, void *stream);
 
+/* ---- attention over the neighbours -----------------------------------------
+ * No counterpart in the reference (its aggregation weights are the fixed entries
+ * of A_hat, gcn/layers.py:219); the learned-weight sibling of that product.
+ * For every row i of the pattern `a`, query head h and the key head h' that it
+ * shares (h' = h / (n_heads / n_kv_heads)), over the edges (i, j) that take part:
+ *   s(i,j) = scale * <q[i,h], k[j,h']> + (use_values ? a->val of the edge : 0)
+ *   out[i,h] = sum_j softmax_j(s(i,j)) v[j,h']
+ * An edge takes no part if edge_mask (nullable, one byte per edge at
+ * edge_mask[mask_index ? mask_index[slot] : slot]) is 0 there or its value is
+ * -inf: its rows of k and v are not read for it.  A row without an edge that takes
+ * part gives zeros.  Operands: dtype elements, q [n_rows, n_heads, head_dim],
+ * k and v [n_cols, n_kv_heads, head_dim], rows of head_dim (1..256) contiguous
+ * elements, other strides in elements (0 allowed, not negative).  Logits, softmax
+ * and sums are fp32, results are rounded once.  Sums have a fixed order: results
+ * are bitwise reproducible.
+ * Rows of more than 512 edges are cut into pieces joined by a second launch.
+ * max_row_nnz, the most edges of a row, says that there are none (0: unknown); it
+ * never changes a result beyond that order of sums. */
+typedef enum gcnx_dtype { GCNX_F32 = 0, GCNX_BF16 = 1, GCNX_F16 = 2 } gcnx_dtype;
+typedef struct gcnx_attention {
+  const gcnx_csr *a;
+  int32_t use_values;
+  int32_t dtype;              /* gcnx_dtype of q, k, v, out and all gradients */
+  const uint8_t *edge_mask;   /* nullable */
+  const int64_t *mask_index;  /* nullable */
+  int64_t max_row_nnz;        /* 0: unknown */
+  int32_t n_heads, n_kv_heads, head_dim;
+  float scale;
+  const void *q;
+  int64_t q_row, q_head;      /* strides in elements */
+  const void *k;
+  int64_t k_row, k_head;
+  const void *v;
+  int64_t v_row, v_head;
+} gcnx_attention;
+/* stats (nullable, fp32 [n_rows, n_heads, 2]): the row's largest logit and one over
+ * the sum of exp(s - it) (0, 0 for a row of zeros): what the backward needs. */
+size_t gcnx_attention_workspace_bytes(const gcnx_attention *p);
+int gcnx_attention_forward(const gcnx_attention *p, const int32_t *chunk_row,
+                           void *out, int64_t out_row, int64_t out_head,
+                           float *stats, void *ws, size_t ws_bytes, void *stream);
+/* Gradients of the above for the gradient `dout` of its output, from `out` and
+ * `stats`; the probabilities are formed again.  `at` is the exact transpose of
+ * p->a with its own chunk table, mask index and longest row.  dq [n_rows, n_heads,
+ * head_dim], dk, dv [n_cols, n_kv_heads, head_dim] (summed over the heads that share
+ * them) are contiguous; dq alone or dk and dv alone may be asked for (the others
+ * NULL).  The values and the mask get no gradient. */
+size_t gcnx_attention_backward_workspace_bytes(const gcnx_attention *p, int64_t t_max_row_nnz);
+int gcnx_attention_backward(const gcnx_attention *p, const int32_t *chunk_row,
+                            const gcnx_csr *at, const int32_t *t_chunk_row,
+                            const int64_t *t_mask_index, int64_t t_max_row_nnz,
+                            const void *out, int64_t out_row, int64_t out_head,
+                            const float *stats, const void *dout, int64_t dout_row,
+                            int64_t dout_head, void *dq, void *dk, void *dv,
+                            void *ws, size_t ws_bytes, void *stream);
+
 /* ---- glue kernels of one training step ------------------------------------ */
 
 /* replaces: masked_softmax_cross_entropy + masked_accuracy, gcn/metrics.py:4-20.

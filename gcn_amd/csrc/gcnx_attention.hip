@@ -142,7 +142,7 @@ __device__ __forceinline__ bool find_task(const AttnArgs &p, int heads, Task &t)
       t.row = p.chunk_row[next / kChunkUnit];
       t.beg = p.row_ptr[t.row];
       t.end = p.row_ptr[t.row + 1];
-      if (t.beg < first || t.end - t.beg <= kSegment) return false;
+      if (t.beg < first || t.beg >= next || t.end - t.beg <= kSegment) return false;
       t.end = next;
     } else {                    // the cut row that goes on into this chunk
       t.row = p.chunk_row[first / kChunkUnit];
@@ -293,7 +293,7 @@ __device__ __forceinline__ bool find_cut_row(const AttnArgs &p, int64_t &row, in
   if (next >= p.nnz) return false;
   row = p.chunk_row[next / kChunkUnit];
   const int64_t beg = p.row_ptr[row], end = p.row_ptr[row + 1];
-  if (beg < first || end - beg <= kSegment) return false;
+  if (beg < first || beg >= next || end - beg <= kSegment) return false;
   last = (end - 1) / kSegment;
   return true;
 }
@@ -343,28 +343,57 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
 
 // Row pass of the backward: delta, dq.  Writes m, r, delta side by side for the
 // column pass.
-template <typename T, int LPH, bool WIDE>
-__global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArgs p) {
-  constexpr int N = Piece<T>::N;
-  Task t;
-  if (!find_task<T, LPH>(p, p.heads, t)) return;
-  const int kv = t.head / p.group, n_row = t.write ? t.n : 0;
-  float q[N], g[N], o[N], acc[N] = {};
-  widen<T>(load_piece<T, WIDE>((const T *)p.q + t.row * p.q_row + t.head * p.q_head + t.d0, n_row), q);
-  widen<T>(load_piece<T, WIDE>((const T *)p.dout + t.row * p.dout_row + t.head * p.dout_head + t.d0, n_row), g);
-  widen<T>(load_piece<T, WIDE>((const T *)p.out + t.row * p.out_row + t.head * p.out_head + t.d0, n_row), o);
-  float delta = 0.0f;
+//
+// delta from the stored output carries that output's rounding, which in 16 bits is
+// larger than the differences <dout, v_j> - delta of a row whose values are alike.
+// So <dout, out> is only a first value d0; the pass sums what it is off by,
+//   rest = sum_j p (<dout, v_j> - d0),   and beside  A = sum_j p (<dout, v_j> - d0) k_j
+// also B = sum_j p k_j:  delta = d0 + rest,  dq = scale (A - rest B).
+template <typename T>
+constexpr bool kCorrected = sizeof(T) == 2;
+
+template <typename T, bool WIDE, int N>
+__device__ __forceinline__ void finish_rows(const AttnArgs &p, const Task &t, float m, float r, float d0, float rest,
+                                            float (&a)[N], const float (&b)[N]) {
+  if (t.d0 == 0) p.stats4[t.row * p.heads + t.head] = f32x4{m, r, d0 + rest, 0.0f};
+  if (!p.o0) return;
 #pragma unroll
-  for (int i = 0; i < N; ++i) delta = fmaf(g[i], o[i], delta);
-  delta = group_sum<LPH>(delta);
-  float m = 0.0f, r = 0.0f;
+  for (int i = 0; i < N; ++i) a[i] = (kCorrected<T> ? fmaf(-rest, b[i], a[i]) : a[i]) * p.scale;
+  store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, a);
+}
+
+// What a row's lanes hold of it in the row pass.
+template <typename T, int LPH, bool WIDE>
+__device__ __forceinline__ void load_row(const AttnArgs &p, const Task &t, float (&g)[Piece<T>::N], float &m, float &r, float &d0) {
+  constexpr int N = Piece<T>::N;
+  const int n = t.write ? t.n : 0;
+  float o[N];
+  widen<T>(load_piece<T, WIDE>((const T *)p.dout + t.row * p.dout_row + t.head * p.dout_head + t.d0, n), g);
+  widen<T>(load_piece<T, WIDE>((const T *)p.out + t.row * p.out_row + t.head * p.out_head + t.d0, n), o);
+  d0 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) d0 = fmaf(g[i], o[i], d0);
+  d0 = group_sum<LPH>(d0);
+  m = r = 0.0f;
   if (t.write && t.head < p.heads) {
     const float *st = p.stats + (t.row * p.heads + t.head) * 2;
     m = st[0];
     r = st[1];
   }
+  if (r == 0.0f) d0 = 0.0f;     // a row of zeros hands nothing on, whatever its gradient holds
+}
+
+template <typename T, int LPH, bool WIDE>
+__global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArgs p) {
+  constexpr int N = Piece<T>::N;
+  Task t;
+  if (!find_task<T, LPH>(p, p.heads, t)) return;
+  const int kv = t.head / p.group;
+  float q[N], g[N], acc[N] = {}, low[N] = {}, m, r, d0, rest = 0.0f;
+  widen<T>(load_piece<T, WIDE>((const T *)p.q + t.row * p.q_row + t.head * p.q_head + t.d0, t.write ? t.n : 0), q);
+  load_row<T, LPH, WIDE>(p, t, g, m, r, d0);
   const T *kb = (const T *)p.k + kv * p.k_head + t.d0, *vb = (const T *)p.v + kv * p.v_head + t.d0;
-  if (!p.o0) t.end = t.beg;     // delta alone is asked for
+  if (!kCorrected<T> && !p.o0) t.end = t.beg;      // delta alone is asked for
   for (int64_t e = t.beg + t.edge; e < t.end; e += kUnroll * t.edges) {
     int32_t col[kUnroll];
     float shift[kUnroll];
@@ -387,28 +416,38 @@ __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArg
       }
       s = group_sum<LPH>(s);
       d = group_sum<LPH>(d);
-      const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r * (d - delta) : 0.0f;
+      const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r : 0.0f;
+      const float ds = on[u] ? w * (d - d0) : 0.0f;
+      rest += ds;
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = fmaf(w, (float)k[u][i], acc[i]);
+      for (int i = 0; i < N; ++i) {
+        acc[i] = fmaf(ds, (float)k[u][i], acc[i]);
+        if constexpr (kCorrected<T>) low[i] = fmaf(w, (float)k[u][i], low[i]);
+      }
     }
   }
   for (int at = 1; at < t.edges; at <<= 1) {
     const int off = (LPH * at) << p.slot_heads_log2;
+    rest += __shfl_xor(rest, off, kWave);
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] += __shfl_xor(acc[i], off, kWave);
+    for (int i = 0; i < N; ++i) {
+      acc[i] += __shfl_xor(acc[i], off, kWave);
+      if constexpr (kCorrected<T>) low[i] += __shfl_xor(low[i], off, kWave);
+    }
   }
+  if (!kCorrected<T>) rest = 0.0f;
   if (t.edge != 0 || !t.write || t.n <= 0) return;
-  if (t.d0 == 0 && (t.piece < 0 || (t.piece & 1))) p.stats4[t.row * p.heads + t.head] = f32x4{m, r, delta, 0.0f};
-  if (!p.o0) return;
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (LPH * N);
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * LPH * N + 1);
 #pragma unroll
-    for (int i = 0; i < N; ++i) part[t.d0 + i] = acc[i];
+    for (int i = 0; i < N; ++i) {
+      part[t.d0 + i] = acc[i];
+      part[LPH * N + t.d0 + i] = low[i];
+    }
+    if (t.d0 == 0) part[2 * LPH * N] = rest;
     return;
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] *= p.scale;
-  store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, acc);
+  finish_rows<T, WIDE>(p, t, m, r, d0, rest, acc, low);
 }
 
 // Column pass: a row of the transpose is a column j of the pattern.  The lanes own
@@ -473,7 +512,7 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
   }
   if (t.edge != 0 || !t.write || t.n <= 0) return;
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * LPH * N);
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * LPH * N + 1);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       part[t.d0 + i] = dk[i];
@@ -487,47 +526,62 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
   store_piece<T, WIDE>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, t.n, dv);
 }
 
-// Adds the pieces of cut rows in the backward passes: PARTS vectors a head (dq, or
-// dk and dv), the first of them times scale.
-template <typename T, int LPH, bool WIDE, int PARTS>
+// Adds the pieces of cut rows in the backward passes: two vectors and a number a
+// head (A, B and rest of the row pass; dk, dv and nothing of the column pass).
+template <typename T, int LPH, bool WIDE, bool COLUMNS>
 __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
-  __shared__ float sh[kBlock][PARTS * N + 1];
-  int64_t row, last;
-  if (!find_cut_row(p, row, last)) return;
-  const int heads = PARTS == 2 ? p.kv_heads : p.heads;
+  __shared__ float sh[kBlock][2 * N + 1];
+  Task t;
+  int64_t last;
+  if (!find_cut_row(p, t.row, last)) return;
+  const int heads = COLUMNS ? p.kv_heads : p.heads;
   const int lane = threadIdx.x & (kWave - 1);
   const int piece = lane % LPH, slot = lane / LPH, hs = slot & ((1 << p.slot_heads_log2) - 1);
   const int per_wave = (kWave / LPH) >> p.slot_heads_log2, groups = per_wave * kWavesPerBlock;
   const int group = (slot >> p.slot_heads_log2) + per_wave * (threadIdx.x >> 6);
-  const int head = ((int)blockIdx.y << p.slot_heads_log2) + hs, d0 = piece * N;
-  const int n = head < heads ? p.dim - d0 : 0;
-  float acc[PARTS][N] = {};
-  if (n > 0)
+  t.head = ((int)blockIdx.y << p.slot_heads_log2) + hs;
+  t.d0 = piece * N;
+  t.n = t.head < heads ? p.dim - t.d0 : 0;
+  t.write = true;
+  float a[N] = {}, b[N] = {}, rest = 0.0f;
+  if (t.n > 0)
     for (int64_t c = blockIdx.x + group; c <= last; c += groups) {
-      const float *part = p.part + (c * 2 + (c == blockIdx.x)) * p.part_floats + (int64_t)head * (PARTS * LPH * N);
+      const float *part = p.part + (c * 2 + (c == blockIdx.x)) * p.part_floats + (int64_t)t.head * (2 * LPH * N + 1);
 #pragma unroll
-      for (int x = 0; x < PARTS; ++x)
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[x][i] += part[x * LPH * N + d0 + i];
+      for (int i = 0; i < N; ++i) {
+        a[i] += part[t.d0 + i];
+        b[i] += part[LPH * N + t.d0 + i];
+      }
+      if (!COLUMNS) rest += part[2 * LPH * N];
     }
 #pragma unroll
-  for (int x = 0; x < PARTS; ++x)
-#pragma unroll
-    for (int i = 0; i < N; ++i) sh[threadIdx.x][x * N + i] = acc[x][i];
-  __syncthreads();
-  if (group != 0 || n <= 0) return;
-  for (int g = 1; g < groups; ++g) {
-    const float *other = sh[(g / per_wave) * kWave + (((g % per_wave) << p.slot_heads_log2) + hs) * LPH + piece];
-#pragma unroll
-    for (int x = 0; x < PARTS; ++x)
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[x][i] += other[x * N + i];
+  for (int i = 0; i < N; ++i) {
+    sh[threadIdx.x][i] = a[i];
+    sh[threadIdx.x][N + i] = b[i];
   }
+  sh[threadIdx.x][2 * N] = rest;
+  float g[N], m, r, d0;
+  if (!COLUMNS && group == 0) load_row<T, LPH, WIDE>(p, t, g, m, r, d0);
+  __syncthreads();
+  if (group != 0 || t.n <= 0) return;
+  for (int o = 1; o < groups; ++o) {
+    const float *other = sh[(o / per_wave) * kWave + (((o % per_wave) << p.slot_heads_log2) + hs) * LPH + piece];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[0][i] *= p.scale;
-  store_piece<T, WIDE>((T *)p.o0 + row * p.o0_row + head * p.o0_head + d0, n, acc[0]);
-  if constexpr (PARTS == 2) store_piece<T, WIDE>((T *)p.o1 + row * p.o1_row + head * p.o1_head + d0, n, acc[PARTS - 1]);
+    for (int i = 0; i < N; ++i) {
+      a[i] += other[i];
+      b[i] += other[N + i];
+    }
+    rest += other[2 * N];
+  }
+  if constexpr (COLUMNS) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] *= p.scale;
+    store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, a);
+    store_piece<T, WIDE>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, t.n, b);
+  } else {
+    finish_rows<T, WIDE>(p, t, m, r, d0, rest, a, b);
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -545,7 +599,7 @@ static int lanes_per_head(int dtype, int dim) {
 
 static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim) {
   const int64_t wide = (int64_t)lanes_per_head(dtype, dim) * (dtype == GCNX_F32 ? 4 : 8);
-  return pass == kForward ? heads * (wide + 2) : pass == kBackwardRows ? heads * wide : kv_heads * 2 * wide;
+  return pass == kForward ? heads * (wide + 2) : (pass == kBackwardRows ? heads : kv_heads) * (2 * wide + 1);
 }
 
 static bool rows_are_cut(int64_t nnz, int64_t max_row_nnz) {
@@ -573,10 +627,10 @@ static void launch_pass(int pass, AttnArgs p, hipStream_t stream) {
     if (p.n_pieces) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH, WIDE>), joins, dim3(kBlock), 0, stream, p);
   } else if (pass == kBackwardRows) {
     hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, WIDE>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces && p.o0) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, WIDE, 1>), joins, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, WIDE, false>), joins, dim3(kBlock), 0, stream, p);
   } else {
     hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, WIDE>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, WIDE, 2>), joins, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, WIDE, true>), joins, dim3(kBlock), 0, stream, p);
   }
 }
 

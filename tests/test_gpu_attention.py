@@ -95,7 +95,7 @@ def test_pattern_shapes(env, n_rows, n_cols, nnz):
 
 
 @pytest.mark.parametrize("edges", [510, 511, 512, 513, 514, 1023, 1024, 1025, 2300])
-@pytest.mark.parametrize("before", [0, 1, 511, 700])
+@pytest.mark.parametrize("before", [0, 1, 511, 512, 700, 1024])
 def test_long_rows(env, edges, before):
     """A row cut at multiples of 512 in the order of the nonzeros, and the column of
     the same length in the transpose, at every place relative to the cuts."""

@@ -24,41 +24,83 @@ namespace gcnx {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// A lane's piece of one head's vector: 16 bytes.
+// A lane's piece of one head's vector: 16 bytes.  A head is spread over LPH lanes;
+// where the head is no multiple of the piece, the last piece overlaps the one
+// before it instead of reaching over the head's end: a lane multiplies its elements
+// `skip`.. only, and writes the others with the same values as their owner.  LPH 0:
+// heads shorter than a piece, one lane each, read element by element.
 template <typename T> struct Piece;
 template <> struct Piece<float> { typedef f32x4 raw; static constexpr int N = 4; };
 template <> struct Piece<__bf16> { typedef bf16x8 raw; static constexpr int N = 8; };
 template <> struct Piece<_Float16> { typedef f16x8 raw; static constexpr int N = 8; };
 
-// `n` elements at p (n <= 0: none) into the piece, zeros behind them.  WIDE: p is
-// 16-byte aligned and n is either >= the piece or <= 0.
-template <typename T, bool WIDE>
-__device__ __forceinline__ typename Piece<T>::raw load_piece(const T *p, int n) {
-  typename Piece<T>::raw x = {};
-  if constexpr (WIDE) {
-    if (n > 0) x = *reinterpret_cast<const typename Piece<T>::raw *>(p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i)
-      if (i < n) x[i] = p[i];
-  }
-  return x;
+// Addresses are kept as numbers and turned into pointers to global memory where
+// they are read: base + column * stride is one 32 x 32 + 64 bit multiply-add, and a
+// choice between two addresses does not become a generic (flat) access.
+typedef uint64_t Address;
+#define GCNX_GLOBAL __attribute__((address_space(1)))
+template <typename V>
+__device__ __forceinline__ V load_at(Address a) {
+  return *(const GCNX_GLOBAL V *)a;
+}
+__device__ __forceinline__ Address row_at(Address base, int32_t row, uint32_t stride) {
+  return base + (uint64_t)(uint32_t)row * stride;
 }
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void store_piece(T *p, int n, const float (&v)[Piece<T>::N]) {
-  if constexpr (WIDE) {
-    if (n > 0) {
-      typename Piece<T>::raw x;
+// What lanes without an edge read: loads are never conditional (a load under a
+// branch is waited for before the next one can be issued into its registers).
+__device__ const f32x4 g_zeros[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+
+__device__ __forceinline__ Address at_or_zeros(Address a, bool on) { return on ? a : (Address)&g_zeros[0]; }
+
+// One piece.  Rows need only their elements' alignment: global loads of 16 bytes
+// take any address.  NARROW: `dim` < a piece, the rest repeats the last element.
+template <typename T, bool NARROW>
+__device__ __forceinline__ typename Piece<T>::raw load_piece(Address a, int dim) {
+  typedef typename Piece<T>::raw raw;
+  typedef raw anywhere __attribute__((aligned(sizeof(T))));
+  if constexpr (!NARROW) {
+    return load_at<anywhere>(a);
+  } else {
+    raw x;
 #pragma unroll
-      for (int i = 0; i < Piece<T>::N; ++i) x[i] = (T)v[i];
-      *reinterpret_cast<typename Piece<T>::raw *>(p) = x;
+    for (int i = 0; i < Piece<T>::N; ++i) x[i] = load_at<T>(a + sizeof(T) * (i < dim ? i : dim - 1));
+    return x;
+  }
+}
+
+// <a, b> + c over a piece.  16 bits: two exact products and their sum an instruction.
+template <typename T>
+__device__ __forceinline__ float dot_piece(const typename Piece<T>::raw &a, const typename Piece<T>::raw &b) {
+  float d = 0.0f;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d = fmaf(a[i], b[i], d);
+  } else {
+    typedef T pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const pair x = {a[2 * i], a[2 * i + 1]}, y = {b[2 * i], b[2 * i + 1]};
+      if constexpr (sizeof(T) == 2 && __is_same(T, _Float16)) d = __builtin_amdgcn_fdot2(x, y, d, false);
+      else d = __builtin_amdgcn_fdot2_f32_bf16(x, y, d, false);
     }
+  }
+  return d;
+}
+
+template <typename T, bool NARROW>
+__device__ __forceinline__ void store_piece(T *p, int dim, const float (&v)[Piece<T>::N]) {
+  if constexpr (!NARROW) {
+    typename Piece<T>::raw x;
+#pragma unroll
+    for (int i = 0; i < Piece<T>::N; ++i) x[i] = (T)v[i];
+    __builtin_memcpy(p, &x, sizeof(x));
   } else {
 #pragma unroll
     for (int i = 0; i < Piece<T>::N; ++i)
-      if (i < n) p[i] = (T)v[i];
+      if (i < dim) p[i] = (T)v[i];
   }
 }
 
@@ -82,9 +124,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ bool is_lowest(float x) { return x == -__builtin_inff(); }
 
-// Rows longer than this are cut at the multiples of it in the order of the
-// nonzeros, a wavefront per piece, and joined by a second kernel.
-constexpr int kSegment = 512;
 constexpr int kUnroll = 4;   // edges in flight per lane
 
 struct AttnArgs {
@@ -99,6 +138,7 @@ struct AttnArgs {
   // operands; strides in elements
   const void *q, *k, *v, *out, *dout;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, dout_row, dout_head;
+  uint32_t q_bytes, q_head_bytes, k_bytes, v_bytes, dout_bytes, dout_head_bytes;   // the same strides where rows are gathered
   int32_t heads, kv_heads, group, dim;
   float scale;
   // results
@@ -109,89 +149,137 @@ struct AttnArgs {
   // work split
   float *part;                  // partial results of cut rows
   int64_t part_floats;          // per piece
-  int64_t n_pieces;             // 2 * chunks of kSegment nonzeros, 0: no row is cut
-  int32_t slot_heads_log2;      // heads side by side in a wavefront
+  int64_t n_pieces;             // 2 * chunks of `segment` nonzeros, 0: no row is cut
+  int32_t segment;              // rows longer than this are cut at its multiples
+  int32_t heads_log2;           // heads side by side in a wavefront (a tile)
   int32_t edge_log2, row_log2;  // edges of a row, rows side by side in a wavefront
+  int32_t tiles, tiles_log2;    // tiles_log2 < 0: no power of two up to 8
 };
 
 // What one group of lanes works on.
 struct Task {
-  int64_t row, beg, end;
+  int64_t row, beg;
+  uint32_t count;               // edges from beg on
   int64_t piece;                // >= 0: a piece of a cut row
-  bool write;
+  bool live;                    // the lane has a head and a row to write
   int32_t edge, edges;          // this lane's place among the edges side by side
-  int32_t head, d0, n;          // head, first element and elements of the lane's piece
+  int32_t head, d0, skip;       // head, first element of the lane's piece, elements counted by another lane
 };
+
+// Tile of heads and place in its list of tasks.  Workgroups go to the 8 dies in
+// turn; tiles are dealt so that a die sees one tile only (or as few as there are):
+// its L2 then holds the operand rows of that tile's heads alone.
+__device__ __forceinline__ int64_t tile_of(const AttnArgs &p, int &tile) {
+  const uint32_t id = blockIdx.x;
+  if (p.tiles_log2 >= 0) {
+    const uint32_t die = id & 7;
+    tile = die & (p.tiles - 1);
+    return ((int64_t)(id >> 3) << (3 - p.tiles_log2)) + (die >> p.tiles_log2);
+  }
+  tile = id % p.tiles;
+  return id / p.tiles;
+}
+
+template <typename T, int LPH>
+__device__ __forceinline__ void place_lane(const AttnArgs &p, int heads, int tile, Task &t, int &slot) {
+  constexpr int L = LPH ? LPH : 1, N = Piece<T>::N;
+  const int lane = threadIdx.x & (kWave - 1), piece = lane % L;
+  slot = lane / L;
+  t.head = (tile << p.heads_log2) + (slot & ((1 << p.heads_log2) - 1));
+  t.d0 = piece * N;
+  t.skip = 0;
+  t.live = t.head < heads && t.d0 < p.dim;
+  if (LPH && t.d0 + N > p.dim) {
+    t.skip = t.d0 < p.dim ? t.d0 + N - p.dim : N;
+    t.d0 = p.dim - N;
+  }
+  slot >>= p.heads_log2;
+}
 
 template <typename T, int LPH>
 __device__ __forceinline__ bool find_task(const AttnArgs &p, int heads, Task &t) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t task = (int64_t)blockIdx.x * kWavesPerBlock + (threadIdx.x >> 6);
-  const int piece = lane % LPH, slot = lane / LPH;
-  const int hs = slot & ((1 << p.slot_heads_log2) - 1);
-  int rest = slot >> p.slot_heads_log2;
-  t.head = ((int)blockIdx.y << p.slot_heads_log2) + hs;
-  t.d0 = piece * Piece<T>::N;
-  t.n = t.head < heads ? p.dim - t.d0 : 0;
+  constexpr int L = LPH ? LPH : 1;
+  int tile, slot;
+  const int64_t task = tile_of(p, tile) * kWavesPerBlock + (threadIdx.x >> 6);
+  place_lane<T, LPH>(p, heads, tile, t, slot);
+  int64_t end;
   if (task < p.n_pieces) {
-    t.edge = rest;
-    t.edges = (kWave / LPH) >> p.slot_heads_log2;
-    const int64_t first = (task >> 1) * kSegment, next = first + kSegment;
+    t.edge = slot;
+    t.edges = (kWave / L) >> p.heads_log2;
+    const int64_t first = (task >> 1) * p.segment, next = first + p.segment;
     if (task & 1) {             // the cut row that begins in this chunk
       if (next >= p.nnz) return false;
       t.row = p.chunk_row[next / kChunkUnit];
       t.beg = p.row_ptr[t.row];
-      t.end = p.row_ptr[t.row + 1];
-      if (t.beg < first || t.beg >= next || t.end - t.beg <= kSegment) return false;
-      t.end = next;
+      end = p.row_ptr[t.row + 1];
+      if (t.beg < first || t.beg >= next || end - t.beg <= p.segment) return false;
+      end = next;
     } else {                    // the cut row that goes on into this chunk
       t.row = p.chunk_row[first / kChunkUnit];
       t.beg = p.row_ptr[t.row];
-      t.end = p.row_ptr[t.row + 1];
-      if (t.beg >= first || t.end - t.beg <= kSegment) return false;
+      end = p.row_ptr[t.row + 1];
+      if (t.beg >= first || end - t.beg <= p.segment) return false;
       t.beg = first;
-      t.end = t.end < next ? t.end : next;
+      end = end < next ? end : next;
     }
     t.piece = task;
-    t.write = true;
   } else {
-    t.edge = rest & ((1 << p.edge_log2) - 1);
+    t.edge = slot & ((1 << p.edge_log2) - 1);
     t.edges = 1 << p.edge_log2;
-    t.row = ((task - p.n_pieces) << p.row_log2) + (rest >> p.edge_log2);
+    t.row = ((task - p.n_pieces) << p.row_log2) + (slot >> p.edge_log2);
     t.piece = -1;
-    t.write = t.row < p.n_rows;
-    t.beg = t.write ? p.row_ptr[t.row] : 0;
-    t.end = t.write ? p.row_ptr[t.row + 1] : 0;
-    if (p.n_pieces && t.end - t.beg > kSegment) {
-      t.write = false;
-      t.end = t.beg;
+    const bool there = t.row < p.n_rows;
+    if (!there) t.row = p.n_rows - 1;
+    t.beg = p.row_ptr[t.row];
+    end = p.row_ptr[t.row + 1];
+    if (!there || (p.n_pieces && end - t.beg > p.segment)) {
+      t.live = false;
+      end = t.beg;            // for every lane of the group: its sums need them all
     }
   }
+  t.count = (uint32_t)(end - t.beg);
   return true;
 }
 
-// One edge: its column, its logit shift, whether it takes part.  An edge whose
-// shift is -inf is out of the softmax like a masked one: its operands are not read,
-// so infinities and NaN in masked places stay where they are.
-__device__ __forceinline__ bool load_edge(const AttnArgs &p, int64_t e, int64_t end, int32_t &col, float &shift) {
-  col = 0;
-  shift = 0.0f;
-  bool on = e < end;
-  if (on) {
+// The edges of the next turn, read one turn ahead: their columns, logit shifts, and
+// whether they take part.  An edge whose shift is -inf is out of the softmax like a
+// masked one: its operands are not read, so infinities and NaN in masked places
+// stay where they are.  SHIFTS: there are values or a mask.
+template <bool SHIFTS>
+struct Edge {
+  int32_t col;
+  float shift;
+  bool on;
+  __device__ __forceinline__ void read(const AttnArgs &p, const Task &t, uint32_t x) {
+    on = x < t.count;
+    const int64_t e = t.beg + (on ? x : 0);       // t.count > 0: edge 0 is there
     col = p.col_idx[e];
-    if (p.val) {
-      shift = p.val[e];
-      on = !is_lowest(shift);
+    shift = 0.0f;
+    if constexpr (SHIFTS) {
+      if (p.val) {
+        shift = p.val[e];
+        on = on && !is_lowest(shift);
+      }
+      if (p.mask) on = on && p.mask[p.mask_index ? p.mask_index[e] : e] != 0;
     }
-    if (p.mask) on = on && p.mask[p.mask_index ? p.mask_index[e] : e] != 0;
   }
-  return on;
+};
+
+// The lane's own operand; elements that another lane counts are zero.
+template <typename T, int LPH>
+__device__ __forceinline__ typename Piece<T>::raw load_own(const AttnArgs &p, const Task &t, const void *base, int64_t row, int64_t head) {
+  const Address at = (Address)((const T *)base + t.row * row + t.head * head + t.d0);
+  typename Piece<T>::raw x = load_piece<T, LPH == 0>(at_or_zeros(at, t.live), p.dim);
+#pragma unroll
+  for (int i = 0; i < Piece<T>::N; ++i)
+    if (LPH ? i < t.skip : i >= p.dim) x[i] = (T)0.0f;
+  return x;
 }
 
-template <typename T>
-__device__ __forceinline__ void widen(const typename Piece<T>::raw &x, float (&f)[Piece<T>::N]) {
-#pragma unroll
-  for (int i = 0; i < Piece<T>::N; ++i) f[i] = (float)x[i];
+// Nothing moves across: what is read ahead stays ahead of the sums.
+__device__ __forceinline__ void read_ahead_fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // Joins two softmax states (m, l, acc); m = -inf: nothing summed yet.
@@ -205,76 +293,84 @@ __device__ __forceinline__ void join(float &m, float &l, float (&acc)[N], float 
   for (int i = 0; i < N; ++i) acc[i] = acc[i] * a + acc2[i] * b;
 }
 
-template <typename T, bool WIDE, int N>
+template <typename T, int LPH, int N>
 __device__ __forceinline__ void finish_forward(const AttnArgs &p, const Task &t, float m, float l, const float (&acc)[N]) {
   const float r = l == 0.0f ? 0.0f : 1.0f / l;      // nothing takes part: zeros
   float o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = acc[i] * r;
-  store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, o);
-  if (p.stats && t.d0 == 0 && t.n > 0) {
+  store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, o);
+  if (p.stats && t.d0 == 0) {
     float *st = p.stats + (t.row * p.heads + t.head) * 2;
     st[0] = is_lowest(m) ? 0.0f : m;
     st[1] = r;
   }
 }
 
-template <typename T, int LPH, bool WIDE>
+// Elements of a partial vector of one head in the workspace.
+template <typename T, int LPH>
+constexpr int kPartWide = (LPH ? LPH : 1) * Piece<T>::N;
+
+template <typename T, int LPH, bool SHIFTS>
 __global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
+  typedef typename Piece<T>::raw raw;
   Task t;
   if (!find_task<T, LPH>(p, p.heads, t)) return;
   const int kv = t.head / p.group;
-  float q[N], acc[N] = {};
-  widen<T>(load_piece<T, WIDE>((const T *)p.q + t.row * p.q_row + t.head * p.q_head + t.d0, t.write ? t.n : 0), q);
-  const T *kb = (const T *)p.k + kv * p.k_head + t.d0, *vb = (const T *)p.v + kv * p.v_head + t.d0;
-  float m = -__builtin_inff(), l = 0.0f;
-  for (int64_t e = t.beg + t.edge; e < t.end; e += kUnroll * t.edges) {
-    int32_t col[kUnroll];
-    float s[kUnroll];
-    bool on[kUnroll];
-    typename Piece<T>::raw k[kUnroll], v[kUnroll];
+  const raw q = load_own<T, LPH>(p, t, p.q, p.q_row, p.q_head);
+  float acc[N] = {}, m = -__builtin_inff(), l = 0.0f;
+  const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
+  if (t.count) {
+    Edge<SHIFTS> next[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) on[u] = load_edge(p, e + u * t.edges, t.end, col[u], s[u]);
+    for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, t.edge + u * t.edges);
+    for (uint32_t x = t.edge; x < t.count; x += kUnroll * t.edges) {
+      raw k[kUnroll], v[kUnroll];
+      float s[kUnroll];
+      bool on[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      k[u] = load_piece<T, WIDE>(kb + col[u] * p.k_row, on[u] ? t.n : 0);
-      v[u] = load_piece<T, WIDE>(vb + col[u] * p.v_row, on[u] ? t.n : 0);
-    }
-    float top = m;
+      for (int u = 0; u < kUnroll; ++u) {
+        on[u] = next[u].on;
+        s[u] = next[u].shift;
+        k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, next[u].col, p.k_bytes), on[u] && t.live), p.dim);
+        v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, next[u].col, p.v_bytes), on[u] && t.live), p.dim);
+      }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float d = 0.0f;
+      for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, x + (kUnroll + u) * t.edges);
+      read_ahead_fence();
+      float top = m;
 #pragma unroll
-      for (int i = 0; i < N; ++i) d = fmaf(q[i], (float)k[u][i], d);
-      d = group_sum<LPH>(d);
-      s[u] = on[u] ? fmaf(d, p.scale, s[u]) : -__builtin_inff();
-      top = fmaxf(top, s[u]);
-    }
-    const float safe = is_lowest(top) ? 0.0f : top;
-    const float keep = exp_of(m - safe);
-    m = top;
-    l *= keep;
+      for (int u = 0; u < kUnroll; ++u) {
+        const float d = group_sum<LPH>(dot_piece<T>(q, k[u]));
+        s[u] = on[u] ? fmaf(d, p.scale, s[u]) : -__builtin_inff();
+        top = fmaxf(top, s[u]);
+      }
+      const float safe = is_lowest(top) ? 0.0f : top;
+      const float keep = exp_of(m - safe);
+      m = top;
+      l *= keep;
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] *= keep;
+      for (int i = 0; i < N; ++i) acc[i] *= keep;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const float w = exp_of(s[u] - safe);
-      l += w;
+      for (int u = 0; u < kUnroll; ++u) {
+        const float w = exp_of(s[u] - safe);
+        l += w;
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = fmaf(w, (float)v[u][i], acc[i]);
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(w, (float)v[u][i], acc[i]);
+      }
     }
   }
   for (int at = 1; at < t.edges; at <<= 1) {
-    const int off = (LPH * at) << p.slot_heads_log2;
+    const int off = ((LPH ? LPH : 1) * at) << p.heads_log2;
     float m2 = __shfl_xor(m, off, kWave), l2 = __shfl_xor(l, off, kWave), acc2[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc2[i] = __shfl_xor(acc[i], off, kWave);
     join<N>(m, l, acc, m2, l2, acc2);
   }
-  if (t.edge != 0 || !t.write || t.n <= 0) return;
+  if (t.edge != 0 || !t.live) return;
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (LPH * N + 2);
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (kPartWide<T, LPH> + 2);
 #pragma unroll
     for (int i = 0; i < N; ++i) part[2 + t.d0 + i] = acc[i];
     if (t.d0 == 0) {
@@ -283,42 +379,56 @@ __global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
     }
     return;
   }
-  finish_forward<T, WIDE>(p, t, m, l, acc);
+  finish_forward<T, LPH, N>(p, t, m, l, acc);
 }
 
-// The cut row that begins in chunk blockIdx.x, if there is one: its pieces are
-// slot 1 of that chunk and slot 0 of the chunks after it.
-__device__ __forceinline__ bool find_cut_row(const AttnArgs &p, int64_t &row, int64_t &last) {
-  const int64_t first = (int64_t)blockIdx.x * kSegment, next = first + kSegment;
+// Joining the pieces of cut rows.  A workgroup per chunk and head tile, at work if a
+// cut row begins in the chunk: its pieces are slot 1 of that chunk and slot 0 of the
+// chunks after it.  They are dealt to the lane groups, each joins its own in order,
+// then the groups are joined through LDS in order: a fixed tree.
+struct JoinTask {
+  int64_t first, last;
+  int32_t group, groups, per_wave, heads_log2;
+  __device__ __forceinline__ const float *part(const AttnArgs &p, int64_t c) const {
+    return p.part + (c * 2 + (c == first)) * p.part_floats;
+  }
+  template <int L>
+  __device__ __forceinline__ int thread_of(int g) const {   // the thread of group g with this lane's head and piece
+    const int lane = threadIdx.x & (kWave - 1), low = lane & ((L << heads_log2) - 1);
+    return (g / per_wave) * kWave + (g % per_wave) * (L << heads_log2) + low;
+  }
+};
+
+template <typename T, int LPH>
+__device__ __forceinline__ bool find_join(const AttnArgs &p, int heads, Task &t, JoinTask &j) {
+  constexpr int L = LPH ? LPH : 1;
+  j.first = blockIdx.x;
+  const int64_t first = j.first * p.segment, next = first + p.segment;
   if (next >= p.nnz) return false;
-  row = p.chunk_row[next / kChunkUnit];
-  const int64_t beg = p.row_ptr[row], end = p.row_ptr[row + 1];
-  if (beg < first || beg >= next || end - beg <= kSegment) return false;
-  last = (end - 1) / kSegment;
+  t.row = p.chunk_row[next / kChunkUnit];
+  const int64_t beg = p.row_ptr[t.row], end = p.row_ptr[t.row + 1];
+  if (beg < first || beg >= next || end - beg <= p.segment) return false;
+  j.last = (end - 1) / p.segment;
+  int slot;
+  place_lane<T, LPH>(p, heads, blockIdx.y, t, slot);
+  j.heads_log2 = p.heads_log2;
+  j.per_wave = (kWave / L) >> p.heads_log2;
+  j.groups = j.per_wave * kWavesPerBlock;
+  j.group = slot + j.per_wave * (threadIdx.x >> 6);
   return true;
 }
 
-// Joins the pieces of cut rows.  A workgroup per row and head tile: the pieces are
-// dealt to the lane groups, each joins its own in order, then the groups are joined
-// through LDS in order: a fixed tree.
-template <typename T, int LPH, bool WIDE>
+template <typename T, int LPH>
 __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   __shared__ float sh[kBlock][N + 2];
   Task t;
-  int64_t last;
-  if (!find_cut_row(p, t.row, last)) return;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int piece = lane % LPH, slot = lane / LPH, hs = slot & ((1 << p.slot_heads_log2) - 1);
-  const int per_wave = (kWave / LPH) >> p.slot_heads_log2, groups = per_wave * kWavesPerBlock;
-  const int group = (slot >> p.slot_heads_log2) + per_wave * (threadIdx.x >> 6);
-  t.head = ((int)blockIdx.y << p.slot_heads_log2) + hs;
-  t.d0 = piece * N;
-  t.n = t.head < p.heads ? p.dim - t.d0 : 0;
+  JoinTask j;
+  if (!find_join<T, LPH>(p, p.heads, t, j)) return;
   float m = -__builtin_inff(), l = 0.0f, acc[N] = {};
-  if (t.n > 0)
-    for (int64_t c = blockIdx.x + group; c <= last; c += groups) {
-      const float *part = p.part + (c * 2 + (c == blockIdx.x)) * p.part_floats + (int64_t)t.head * (LPH * N + 2);
+  if (t.live)
+    for (int64_t c = j.first + j.group; c <= j.last; c += j.groups) {
+      const float *part = j.part(p, c) + (int64_t)t.head * (kPartWide<T, LPH> + 2);
       float a2[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) a2[i] = part[2 + t.d0 + i];
@@ -330,15 +440,15 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
 #pragma unroll
   for (int i = 0; i < N; ++i) mine[2 + i] = acc[i];
   __syncthreads();
-  if (group != 0 || t.n <= 0) return;
-  for (int g = 1; g < groups; ++g) {
-    const float *other = sh[(g / per_wave) * kWave + (((g % per_wave) << p.slot_heads_log2) + hs) * LPH + piece];
+  if (j.group != 0 || !t.live) return;
+  for (int g = 1; g < j.groups; ++g) {
+    const float *other = sh[j.thread_of<LPH ? LPH : 1>(g)];
     float a2[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) a2[i] = other[2 + i];
     join<N>(m, l, acc, other[0], other[1], a2);
   }
-  finish_forward<T, WIDE>(p, t, m, l, acc);
+  finish_forward<T, LPH, N>(p, t, m, l, acc);
 }
 
 // Row pass of the backward: delta, dq.  Writes m, r, delta side by side for the
@@ -352,82 +462,73 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
 template <typename T>
 constexpr bool kCorrected = sizeof(T) == 2;
 
-template <typename T, bool WIDE, int N>
+template <typename T, int LPH, int N>
 __device__ __forceinline__ void finish_rows(const AttnArgs &p, const Task &t, float m, float r, float d0, float rest,
                                             float (&a)[N], const float (&b)[N]) {
   if (t.d0 == 0) p.stats4[t.row * p.heads + t.head] = f32x4{m, r, d0 + rest, 0.0f};
   if (!p.o0) return;
 #pragma unroll
   for (int i = 0; i < N; ++i) a[i] = (kCorrected<T> ? fmaf(-rest, b[i], a[i]) : a[i]) * p.scale;
-  store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, a);
+  store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, a);
 }
 
 // What a row's lanes hold of it in the row pass.
-template <typename T, int LPH, bool WIDE>
-__device__ __forceinline__ void load_row(const AttnArgs &p, const Task &t, float (&g)[Piece<T>::N], float &m, float &r, float &d0) {
-  constexpr int N = Piece<T>::N;
-  const int n = t.write ? t.n : 0;
-  float o[N];
-  widen<T>(load_piece<T, WIDE>((const T *)p.dout + t.row * p.dout_row + t.head * p.dout_head + t.d0, n), g);
-  widen<T>(load_piece<T, WIDE>((const T *)p.out + t.row * p.out_row + t.head * p.out_head + t.d0, n), o);
-  d0 = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) d0 = fmaf(g[i], o[i], d0);
-  d0 = group_sum<LPH>(d0);
-  m = r = 0.0f;
-  if (t.write && t.head < p.heads) {
-    const float *st = p.stats + (t.row * p.heads + t.head) * 2;
-    m = st[0];
-    r = st[1];
-  }
-  if (r == 0.0f) d0 = 0.0f;     // a row of zeros hands nothing on, whatever its gradient holds
+template <typename T, int LPH>
+__device__ __forceinline__ typename Piece<T>::raw load_row(const AttnArgs &p, const Task &t, float &m, float &r, float &d0) {
+  const typename Piece<T>::raw g = load_own<T, LPH>(p, t, p.dout, p.dout_row, p.dout_head);
+  const typename Piece<T>::raw o = load_own<T, LPH>(p, t, p.out, p.out_row, p.out_head);
+  const f32x2 st = load_at<f32x2>(at_or_zeros((Address)(p.stats + (t.row * p.heads + t.head) * 2), t.live));
+  m = st[0];
+  r = st[1];
+  d0 = group_sum<LPH>(dot_piece<T>(g, o));
+  return g;
 }
 
-template <typename T, int LPH, bool WIDE>
+template <typename T, int LPH, bool SHIFTS>
 __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
+  typedef typename Piece<T>::raw raw;
   Task t;
   if (!find_task<T, LPH>(p, p.heads, t)) return;
   const int kv = t.head / p.group;
-  float q[N], g[N], acc[N] = {}, low[N] = {}, m, r, d0, rest = 0.0f;
-  widen<T>(load_piece<T, WIDE>((const T *)p.q + t.row * p.q_row + t.head * p.q_head + t.d0, t.write ? t.n : 0), q);
-  load_row<T, LPH, WIDE>(p, t, g, m, r, d0);
-  const T *kb = (const T *)p.k + kv * p.k_head + t.d0, *vb = (const T *)p.v + kv * p.v_head + t.d0;
-  if (!kCorrected<T> && !p.o0) t.end = t.beg;      // delta alone is asked for
-  for (int64_t e = t.beg + t.edge; e < t.end; e += kUnroll * t.edges) {
-    int32_t col[kUnroll];
-    float shift[kUnroll];
-    bool on[kUnroll];
-    typename Piece<T>::raw k[kUnroll], v[kUnroll];
+  float acc[N] = {}, low[N] = {}, m, r, d0, rest = 0.0f;
+  const raw q = load_own<T, LPH>(p, t, p.q, p.q_row, p.q_head), g = load_row<T, LPH>(p, t, m, r, d0);
+  const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
+  if (!kCorrected<T> && !p.o0) t.count = 0;        // delta alone is asked for
+  if (t.count) {
+    Edge<SHIFTS> next[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) on[u] = load_edge(p, e + u * t.edges, t.end, col[u], shift[u]);
+    for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, t.edge + u * t.edges);
+    for (uint32_t x = t.edge; x < t.count; x += kUnroll * t.edges) {
+      raw k[kUnroll], v[kUnroll];
+      float shift[kUnroll];
+      bool on[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      k[u] = load_piece<T, WIDE>(kb + col[u] * p.k_row, on[u] ? t.n : 0);
-      v[u] = load_piece<T, WIDE>(vb + col[u] * p.v_row, on[u] ? t.n : 0);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float s = 0.0f, d = 0.0f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        s = fmaf(q[i], (float)k[u][i], s);
-        d = fmaf(g[i], (float)v[u][i], d);
+      for (int u = 0; u < kUnroll; ++u) {
+        on[u] = next[u].on;
+        shift[u] = next[u].shift;
+        k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, next[u].col, p.k_bytes), on[u] && t.live), p.dim);
+        v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, next[u].col, p.v_bytes), on[u] && t.live), p.dim);
       }
-      s = group_sum<LPH>(s);
-      d = group_sum<LPH>(d);
-      const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r : 0.0f;
-      const float ds = on[u] ? w * (d - d0) : 0.0f;
-      rest += ds;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        acc[i] = fmaf(ds, (float)k[u][i], acc[i]);
-        if constexpr (kCorrected<T>) low[i] = fmaf(w, (float)k[u][i], low[i]);
+      for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, x + (kUnroll + u) * t.edges);
+      read_ahead_fence();
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const float s = group_sum<LPH>(dot_piece<T>(q, k[u])), d = group_sum<LPH>(dot_piece<T>(g, v[u]));
+        const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r : 0.0f;
+        const float ds = on[u] ? w * (d - d0) : 0.0f;
+        rest += ds;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          acc[i] = fmaf(ds, (float)k[u][i], acc[i]);
+          if constexpr (kCorrected<T>) low[i] = fmaf(w, (float)k[u][i], low[i]);
+        }
       }
     }
   }
   for (int at = 1; at < t.edges; at <<= 1) {
-    const int off = (LPH * at) << p.slot_heads_log2;
+    const int off = ((LPH ? LPH : 1) * at) << p.heads_log2;
     rest += __shfl_xor(rest, off, kWave);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -436,124 +537,129 @@ __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArg
     }
   }
   if (!kCorrected<T>) rest = 0.0f;
-  if (t.edge != 0 || !t.write || t.n <= 0) return;
+  if (t.edge != 0 || !t.live) return;
+  if (r == 0.0f) d0 = rest = 0.0f;   // a row of zeros hands nothing on, whatever its gradient holds
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * LPH * N + 1);
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 1);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       part[t.d0 + i] = acc[i];
-      part[LPH * N + t.d0 + i] = low[i];
+      part[kPartWide<T, LPH> + t.d0 + i] = low[i];
     }
-    if (t.d0 == 0) part[2 * LPH * N] = rest;
+    if (t.d0 == 0) part[2 * kPartWide<T, LPH>] = rest;
     return;
   }
-  finish_rows<T, WIDE>(p, t, m, r, d0, rest, acc, low);
+  finish_rows<T, LPH, N>(p, t, m, r, d0, rest, acc, low);
 }
 
 // Column pass: a row of the transpose is a column j of the pattern.  The lanes own
 // the key heads; the edges of the column are walked once per query head that
-// shares the key head, as edges * group items.
-template <typename T, int LPH, bool WIDE>
+// shares the key head, as count * group items.
+template <typename T, int LPH, bool SHIFTS>
 __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
+  typedef typename Piece<T>::raw raw;
   Task t;
   if (!find_task<T, LPH>(p, p.kv_heads, t)) return;
-  const int n_row = t.write ? t.n : 0;
-  float k[N], v[N], dk[N] = {}, dv[N] = {};
-  widen<T>(load_piece<T, WIDE>((const T *)p.k + t.row * p.k_row + t.head * p.k_head + t.d0, n_row), k);
-  widen<T>(load_piece<T, WIDE>((const T *)p.v + t.row * p.v_row + t.head * p.v_head + t.d0, n_row), v);
-  const T *qb = (const T *)p.q + t.d0, *gb = (const T *)p.dout + t.d0;
-  const int64_t items = (t.end - t.beg) * p.group;
-  for (int64_t it = t.edge; it < items; it += kUnroll * t.edges) {
-    int32_t row[kUnroll], head[kUnroll];
-    float shift[kUnroll];
-    bool on[kUnroll];
-    typename Piece<T>::raw q[kUnroll], g[kUnroll];
-    f32x4 st[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t x = it + u * t.edges;
-      const int64_t e = p.group == 1 ? x : items <= 0xffffffffll ? (int64_t)((uint32_t)x / (uint32_t)p.group) : x / p.group;
-      head[u] = t.head * p.group + (int)(x - e * p.group);
-      on[u] = load_edge(p, t.beg + e, t.end, row[u], shift[u]) && t.n > 0;
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      q[u] = load_piece<T, WIDE>(qb + row[u] * p.q_row + head[u] * p.q_head, on[u] ? t.n : 0);
-      g[u] = load_piece<T, WIDE>(gb + row[u] * p.dout_row + head[u] * p.dout_head, on[u] ? t.n : 0);
-      st[u] = on[u] ? p.stats4[(int64_t)row[u] * p.heads + head[u]] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float s = 0.0f, d = 0.0f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        s = fmaf(k[i], (float)q[u][i], s);
-        d = fmaf(v[i], (float)g[u][i], d);
+  float dk[N] = {}, dv[N] = {};
+  const raw k = load_own<T, LPH>(p, t, p.k, p.k_row, p.k_head), v = load_own<T, LPH>(p, t, p.v, p.v_row, p.v_head);
+  const int head0 = t.head * p.group;
+  const Address qb = (Address)((const T *)p.q + head0 * p.q_head + t.d0), gb = (Address)((const T *)p.dout + head0 * p.dout_head + t.d0),
+                stb = (Address)(p.stats4 + head0);
+  if (t.count) {
+    const uint32_t group = p.group;
+    // item x is edge x / group under query head x % group
+    uint32_t at = t.edge / group, sub = t.edge - at * group;
+    const uint32_t at_step = t.edges / group, sub_step = t.edges - at_step * group;
+    Edge<SHIFTS> next[kUnroll];
+    uint32_t next_sub[kUnroll];
+    auto read = [&](int u) {
+      next[u].read(p, t, at);
+      next_sub[u] = sub;
+      at += at_step;
+      sub += sub_step;
+      if (sub >= group) {
+        sub -= group;
+        ++at;
       }
-      s = group_sum<LPH>(s);
-      d = group_sum<LPH>(d);
-      const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - st[u][0]) * st[u][1] : 0.0f;
-      const float ds = on[u] ? w * (d - st[u][2]) : 0.0f;
+    };
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        dv[i] = fmaf(w, (float)g[u][i], dv[i]);
-        dk[i] = fmaf(ds, (float)q[u][i], dk[i]);
+    for (int u = 0; u < kUnroll; ++u) read(u);
+    for (uint32_t first = t.edge / group; first < t.count;) {
+      raw q[kUnroll], g[kUnroll];
+      f32x4 st[kUnroll];
+      float shift[kUnroll];
+      bool on[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        on[u] = next[u].on;
+        shift[u] = next[u].shift;
+        const bool there = on[u] && t.live;
+        const int32_t row = next[u].col, h = next_sub[u];
+        q[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(row_at(qb, row, p.q_bytes), h, p.q_head_bytes), there), p.dim);
+        g[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(row_at(gb, row, p.dout_bytes), h, p.dout_head_bytes), there), p.dim);
+        st[u] = load_at<f32x4>(at_or_zeros(row_at(stb, row, p.heads * 16) + h * 16, there));
+      }
+      first = at;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) read(u);
+      read_ahead_fence();
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const float s = group_sum<LPH>(dot_piece<T>(k, q[u])), d = group_sum<LPH>(dot_piece<T>(v, g[u]));
+        const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - st[u][0]) * st[u][1] : 0.0f;
+        const float ds = on[u] ? w * (d - st[u][2]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          dv[i] = fmaf(w, (float)g[u][i], dv[i]);
+          dk[i] = fmaf(ds, (float)q[u][i], dk[i]);
+        }
       }
     }
   }
   for (int at = 1; at < t.edges; at <<= 1) {
-    const int off = (LPH * at) << p.slot_heads_log2;
+    const int off = ((LPH ? LPH : 1) * at) << p.heads_log2;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       dk[i] += __shfl_xor(dk[i], off, kWave);
       dv[i] += __shfl_xor(dv[i], off, kWave);
     }
   }
-  if (t.edge != 0 || !t.write || t.n <= 0) return;
+  if (t.edge != 0 || !t.live) return;
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * LPH * N + 1);
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 1);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       part[t.d0 + i] = dk[i];
-      part[LPH * N + t.d0 + i] = dv[i];
+      part[kPartWide<T, LPH> + t.d0 + i] = dv[i];
     }
     return;
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) dk[i] *= p.scale;
-  store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, dk);
-  store_piece<T, WIDE>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, t.n, dv);
+  store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, dk);
+  store_piece<T, LPH == 0>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, p.dim, dv);
 }
 
 // Adds the pieces of cut rows in the backward passes: two vectors and a number a
 // head (A, B and rest of the row pass; dk, dv and nothing of the column pass).
-template <typename T, int LPH, bool WIDE, bool COLUMNS>
+template <typename T, int LPH, bool COLUMNS>
 __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   __shared__ float sh[kBlock][2 * N + 1];
   Task t;
-  int64_t last;
-  if (!find_cut_row(p, t.row, last)) return;
-  const int heads = COLUMNS ? p.kv_heads : p.heads;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int piece = lane % LPH, slot = lane / LPH, hs = slot & ((1 << p.slot_heads_log2) - 1);
-  const int per_wave = (kWave / LPH) >> p.slot_heads_log2, groups = per_wave * kWavesPerBlock;
-  const int group = (slot >> p.slot_heads_log2) + per_wave * (threadIdx.x >> 6);
-  t.head = ((int)blockIdx.y << p.slot_heads_log2) + hs;
-  t.d0 = piece * N;
-  t.n = t.head < heads ? p.dim - t.d0 : 0;
-  t.write = true;
+  JoinTask j;
+  if (!find_join<T, LPH>(p, COLUMNS ? p.kv_heads : p.heads, t, j)) return;
   float a[N] = {}, b[N] = {}, rest = 0.0f;
-  if (t.n > 0)
-    for (int64_t c = blockIdx.x + group; c <= last; c += groups) {
-      const float *part = p.part + (c * 2 + (c == blockIdx.x)) * p.part_floats + (int64_t)t.head * (2 * LPH * N + 1);
+  if (t.live)
+    for (int64_t c = j.first + j.group; c <= j.last; c += j.groups) {
+      const float *part = j.part(p, c) + (int64_t)t.head * (2 * kPartWide<T, LPH> + 1);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         a[i] += part[t.d0 + i];
-        b[i] += part[LPH * N + t.d0 + i];
+        b[i] += part[kPartWide<T, LPH> + t.d0 + i];
       }
-      if (!COLUMNS) rest += part[2 * LPH * N];
+      if (!COLUMNS) rest += part[2 * kPartWide<T, LPH>];
     }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -561,12 +667,12 @@ __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArg
     sh[threadIdx.x][N + i] = b[i];
   }
   sh[threadIdx.x][2 * N] = rest;
-  float g[N], m, r, d0;
-  if (!COLUMNS && group == 0) load_row<T, LPH, WIDE>(p, t, g, m, r, d0);
+  float m = 0.0f, r = 0.0f, d0 = 0.0f;
+  if (!COLUMNS && j.group == 0) load_row<T, LPH>(p, t, m, r, d0);
   __syncthreads();
-  if (group != 0 || t.n <= 0) return;
-  for (int o = 1; o < groups; ++o) {
-    const float *other = sh[(o / per_wave) * kWave + (((o % per_wave) << p.slot_heads_log2) + hs) * LPH + piece];
+  if (j.group != 0 || !t.live) return;
+  for (int o = 1; o < j.groups; ++o) {
+    const float *other = sh[j.thread_of<LPH ? LPH : 1>(o)];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       a[i] += other[i];
@@ -577,10 +683,11 @@ __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArg
   if constexpr (COLUMNS) {
 #pragma unroll
     for (int i = 0; i < N; ++i) a[i] *= p.scale;
-    store_piece<T, WIDE>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, t.n, a);
-    store_piece<T, WIDE>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, t.n, b);
+    store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, a);
+    store_piece<T, LPH == 0>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, p.dim, b);
   } else {
-    finish_rows<T, WIDE>(p, t, m, r, d0, rest, a, b);
+    if (r == 0.0f) d0 = rest = 0.0f;
+    finish_rows<T, LPH, N>(p, t, m, r, d0, rest, a, b);
   }
 }
 
@@ -593,76 +700,105 @@ static int log2_ceil(int64_t x) {
   return l;
 }
 
+static int piece_elements(int dtype) { return dtype == GCNX_F32 ? 4 : 8; }
+
+// 0: a head is shorter than a piece
 static int lanes_per_head(int dtype, int dim) {
-  return 1 << log2_ceil(ceil_div(dim, dtype == GCNX_F32 ? 4 : 8));
+  const int n = piece_elements(dtype);
+  return dim < n ? 0 : 1 << log2_ceil(ceil_div(dim, n));
 }
 
 static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim) {
-  const int64_t wide = (int64_t)lanes_per_head(dtype, dim) * (dtype == GCNX_F32 ? 4 : 8);
+  const int lph = lanes_per_head(dtype, dim);
+  const int64_t wide = (int64_t)(lph ? lph : 1) * piece_elements(dtype);
   return pass == kForward ? heads * (wide + 2) : (pass == kBackwardRows ? heads : kv_heads) * (2 * wide + 1);
 }
 
-static bool rows_are_cut(int64_t nnz, int64_t max_row_nnz) {
-  return nnz > kSegment && (max_row_nnz <= 0 || max_row_nnz > kSegment);
+// Edges a wavefront takes of one row at most.
+static int segment_of(int64_t nnz) {
+  (void)nnz;
+  return 512;
 }
 
-template <typename T, int LPH, bool WIDE>
-static void launch_pass(int pass, AttnArgs p, hipStream_t stream) {
+static bool rows_are_cut(int64_t nnz, int64_t max_row_nnz) {
+  return nnz > segment_of(nnz) && (max_row_nnz <= 0 || max_row_nnz > segment_of(nnz) || nnz > 0x7fffffff);
+}
+
+static size_t part_bytes(const gcnx_attention *p, int64_t max_row_nnz, int pass) {
+  const int64_t nnz = p->a->nnz;
+  if (!rows_are_cut(nnz, max_row_nnz)) return 0;
+  return align_up((size_t)(2 * ceil_div(nnz, segment_of(nnz))) *
+                      part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim) * sizeof(float), 256);
+}
+
+static size_t stats4_bytes(const gcnx_attention *p) {
+  return align_up((size_t)p->a->n_rows * p->n_heads * 16, 256);
+}
+
+template <typename T, int LPH, bool SHIFTS>
+static void launch_pass(int pass, const AttnArgs &p, dim3 grid, dim3 joins, hipStream_t stream) {
+  if (pass == kForward) {
+    hipLaunchKernelGGL((attention_forward_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH>), joins, dim3(kBlock), 0, stream, p);
+  } else if (pass == kBackwardRows) {
+    hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, false>), joins, dim3(kBlock), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, true>), joins, dim3(kBlock), 0, stream, p);
+  }
+}
+
+template <typename T, int LPH>
+static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   const int heads = pass == kBackwardColumns ? p.kv_heads : p.heads;
-  const int slots_log2 = log2_ceil(kWave / LPH);
+  const int slots_log2 = log2_ceil(kWave / (LPH ? LPH : 1));
   const int heads_log2 = log2_ceil(heads);
-  p.slot_heads_log2 = heads_log2 < slots_log2 ? heads_log2 : slots_log2;
-  const int spare = slots_log2 - p.slot_heads_log2;
+  p.heads_log2 = heads_log2 < slots_log2 ? heads_log2 : slots_log2;
+  const int spare = slots_log2 - p.heads_log2;
   // edges side by side: about kUnroll per lane at the average row; what is left
   // takes further rows
   const int64_t items = ceil_div(p.nnz * (pass == kBackwardColumns ? p.group : 1), p.n_rows);
-  int e = log2_ceil(ceil_div(items, kUnroll));
+  const int e = log2_ceil(ceil_div(items, kUnroll));
   p.edge_log2 = e < spare ? e : spare;
   p.row_log2 = spare - p.edge_log2;
-  const int64_t tasks = p.n_pieces + ceil_div(p.n_rows, (int64_t)1 << p.row_log2);
-  const dim3 grid((unsigned)ceil_div(tasks, kWavesPerBlock), (unsigned)ceil_div(heads, (int64_t)1 << p.slot_heads_log2));
-  const dim3 joins((unsigned)(p.n_pieces / 2), grid.y);
-  if (pass == kForward) {
-    hipLaunchKernelGGL((attention_forward_kernel<T, LPH, WIDE>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH, WIDE>), joins, dim3(kBlock), 0, stream, p);
-  } else if (pass == kBackwardRows) {
-    hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, WIDE>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, WIDE, false>), joins, dim3(kBlock), 0, stream, p);
-  } else {
-    hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, WIDE>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, WIDE, true>), joins, dim3(kBlock), 0, stream, p);
-  }
-}
-
-template <typename T, bool WIDE>
-static void launch_lanes(int pass, int lph, const AttnArgs &p, hipStream_t stream) {
-  switch (lph) {
-    case 1: return launch_pass<T, 1, WIDE>(pass, p, stream);
-    case 2: return launch_pass<T, 2, WIDE>(pass, p, stream);
-    case 4: return launch_pass<T, 4, WIDE>(pass, p, stream);
-    case 8: return launch_pass<T, 8, WIDE>(pass, p, stream);
-    case 16: return launch_pass<T, 16, WIDE>(pass, p, stream);
-    case 32: return launch_pass<T, 32, WIDE>(pass, p, stream);
-    default:
-      if constexpr (Piece<T>::N == 4) return launch_pass<T, 64, WIDE>(pass, p, stream);
-  }
-}
-
-template <typename T>
-static void launch_type(int pass, bool wide, int lph, const AttnArgs &p, hipStream_t stream) {
-  if (wide) launch_lanes<T, true>(pass, lph, p, stream);
-  else launch_lanes<T, false>(pass, lph, p, stream);
-}
-
-static int launch(int pass, int dtype, bool wide, AttnArgs p, hipStream_t stream) {
-  if (p.n_rows == 0) return GCNX_OK;
-  const int lph = lanes_per_head(dtype, p.dim);
-  if (dtype == GCNX_F32) launch_type<float>(pass, wide, lph, p, stream);
-  else if (dtype == GCNX_BF16) launch_type<__bf16>(pass, wide, lph, p, stream);
-  else launch_type<_Float16>(pass, wide, lph, p, stream);
+  p.tiles = (int)ceil_div(heads, (int64_t)1 << p.heads_log2);
+  p.tiles_log2 = p.tiles <= 8 && (p.tiles & (p.tiles - 1)) == 0 ? log2_ceil(p.tiles) : -1;
+  int64_t blocks = ceil_div(p.n_pieces + ceil_div(p.n_rows, (int64_t)1 << p.row_log2), kWavesPerBlock);
+  blocks = p.tiles_log2 >= 0 ? ceil_div(blocks, 8 >> p.tiles_log2) * 8 : blocks * p.tiles;
+  GCNX_REQUIRE(blocks <= 0x7fffffff && p.n_pieces / 2 <= 0x7fffffff, GCNX_ERR_UNSUPPORTED, "attention: too many rows for one launch");
+  const dim3 grid((unsigned)blocks), joins((unsigned)(p.n_pieces / 2), (unsigned)p.tiles);
+  if (p.val || p.mask) launch_pass<T, LPH, true>(pass, p, grid, joins, stream);
+  else launch_pass<T, LPH, false>(pass, p, grid, joins, stream);
   GCNX_CHECK_LAUNCH();
   return GCNX_OK;
 }
+
+template <typename T>
+static int launch_type(int pass, int lph, const AttnArgs &p, hipStream_t stream) {
+  switch (lph) {
+    case 0: return launch_lanes<T, 0>(pass, p, stream);
+    case 1: return launch_lanes<T, 1>(pass, p, stream);
+    case 2: return launch_lanes<T, 2>(pass, p, stream);
+    case 4: return launch_lanes<T, 4>(pass, p, stream);
+    case 8: return launch_lanes<T, 8>(pass, p, stream);
+    case 16: return launch_lanes<T, 16>(pass, p, stream);
+    case 32: return launch_lanes<T, 32>(pass, p, stream);
+    default:
+      if constexpr (Piece<T>::N == 4) return launch_lanes<T, 64>(pass, p, stream);
+      else return GCNX_ERR_UNSUPPORTED;
+  }
+}
+
+static int launch(int pass, int dtype, const AttnArgs &p, hipStream_t stream) {
+  if (p.n_rows == 0) return GCNX_OK;
+  const int lph = lanes_per_head(dtype, p.dim);
+  return dtype == GCNX_F32 ? launch_type<float>(pass, lph, p, stream)
+         : dtype == GCNX_BF16 ? launch_type<__bf16>(pass, lph, p, stream) : launch_type<_Float16>(pass, lph, p, stream);
+}
+
+// gathered rows are addressed by 32-bit byte strides
+static bool stride_ok(int64_t elements) { return elements >= 0 && elements < (1ll << 30); }
 
 static int check(const gcnx_attention *p) {
   GCNX_REQUIRE(p && p->a, GCNX_ERR_INVALID_ARG, "attention: null argument");
@@ -673,22 +809,16 @@ static int check(const gcnx_attention *p) {
   GCNX_REQUIRE(p->n_kv_heads >= 1 && p->n_heads >= 1 && p->n_heads % p->n_kv_heads == 0 && p->n_heads <= 65535,
                GCNX_ERR_INVALID_ARG, "attention: %d query heads over %d key heads", p->n_heads, p->n_kv_heads);
   GCNX_REQUIRE(p->a->n_rows >= 0 && p->a->n_cols >= 0 && p->a->nnz >= 0 && p->a->n_rows < 2147483647 &&
-                   p->a->nnz / kSegment < 1000000000, GCNX_ERR_INVALID_ARG, "attention: bad matrix size");
+                   p->a->n_cols < 2147483647, GCNX_ERR_INVALID_ARG, "attention: bad matrix size");
   GCNX_REQUIRE((p->a->n_rows == 0 || p->a->row_ptr) && (p->a->nnz == 0 || p->a->col_idx), GCNX_ERR_INVALID_ARG,
                "attention: null matrix array");
   GCNX_REQUIRE(p->a->nnz == 0 || (p->a->n_rows > 0 && p->a->n_cols > 0), GCNX_ERR_INVALID_ARG, "attention: nonzeros in an empty matrix");
   GCNX_REQUIRE(!p->use_values || p->a->nnz == 0 || p->a->val, GCNX_ERR_INVALID_ARG, "attention: values asked for, none given");
   GCNX_REQUIRE((p->a->n_rows == 0 || p->q) && (p->a->n_cols == 0 || (p->k && p->v)), GCNX_ERR_INVALID_ARG,
                "attention: null operand");
-  GCNX_REQUIRE(p->q_row >= 0 && p->q_head >= 0 && p->k_row >= 0 && p->k_head >= 0 && p->v_row >= 0 && p->v_head >= 0,
-               GCNX_ERR_INVALID_ARG, "attention: negative stride");
+  GCNX_REQUIRE(stride_ok(p->q_row) && stride_ok(p->q_head) && stride_ok(p->k_row) && stride_ok(p->k_head) &&
+                   stride_ok(p->v_row) && stride_ok(p->v_head), GCNX_ERR_INVALID_ARG, "attention: a stride outside 0..2^30 - 1");
   return GCNX_OK;
-}
-
-// 16-byte loads of every piece: base and strides multiples of 16 bytes.
-static bool piece_aligned(const gcnx_attention *p, const void *base, int64_t row, int64_t head) {
-  const int64_t n = p->dtype == GCNX_F32 ? 4 : 8;
-  return p->head_dim % n == 0 && row % n == 0 && head % n == 0 && ((uintptr_t)base & 15) == 0;
 }
 
 static AttnArgs common_args(const gcnx_attention *p) {
@@ -696,6 +826,11 @@ static AttnArgs common_args(const gcnx_attention *p) {
   g.q = p->q; g.q_row = p->q_row; g.q_head = p->q_head;
   g.k = p->k; g.k_row = p->k_row; g.k_head = p->k_head;
   g.v = p->v; g.v_row = p->v_row; g.v_head = p->v_head;
+  const int64_t size = p->dtype == GCNX_F32 ? 4 : 2;
+  g.q_bytes = (uint32_t)(p->q_row * size);
+  g.q_head_bytes = (uint32_t)(p->q_head * size);
+  g.k_bytes = (uint32_t)(p->k_row * size);
+  g.v_bytes = (uint32_t)(p->v_row * size);
   g.heads = p->n_heads;
   g.kv_heads = p->n_kv_heads;
   g.group = p->n_heads / p->n_kv_heads;
@@ -716,17 +851,8 @@ static void set_pattern(AttnArgs &g, const gcnx_attention *p, const gcnx_csr *a,
   g.nnz = a->nnz;
   g.part = part;
   g.part_floats = part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim);
-  g.n_pieces = rows_are_cut(a->nnz, max_row_nnz) ? 2 * ceil_div(a->nnz, kSegment) : 0;
-}
-
-static size_t part_bytes(const gcnx_attention *p, int64_t max_row_nnz, int pass) {
-  if (!rows_are_cut(p->a->nnz, max_row_nnz)) return 0;
-  return align_up((size_t)(2 * ceil_div(p->a->nnz, kSegment)) *
-                      part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim) * sizeof(float), 256);
-}
-
-static size_t stats4_bytes(const gcnx_attention *p) {
-  return align_up((size_t)p->a->n_rows * p->n_heads * 16, 256);
+  g.segment = segment_of(a->nnz);
+  g.n_pieces = rows_are_cut(a->nnz, max_row_nnz) ? 2 * ceil_div(a->nnz, g.segment) : 0;
 }
 
 }  // namespace gcnx
@@ -742,7 +868,7 @@ extern "C" int gcnx_attention_forward(const gcnx_attention *p, const int32_t *ch
                                       int64_t out_head, float *stats, void *ws, size_t ws_bytes, void *stream) {
   if (int rc = check(p)) return rc;
   if (p->a->n_rows == 0) return GCNX_OK;
-  GCNX_REQUIRE(out && out_row >= 0 && out_head >= 0, GCNX_ERR_INVALID_ARG, "attention: bad output");
+  GCNX_REQUIRE(out && stride_ok(out_row) && stride_ok(out_head), GCNX_ERR_INVALID_ARG, "attention: bad output");
   const size_t need = part_bytes(p, p->max_row_nnz, kForward);
   GCNX_REQUIRE(need == 0 || (chunk_row && ws && ws_bytes >= need), GCNX_ERR_WORKSPACE,
                "attention: workspace of %zu bytes (and the chunk table) needed, %zu given", need, ws_bytes);
@@ -750,9 +876,7 @@ extern "C" int gcnx_attention_forward(const gcnx_attention *p, const int32_t *ch
   set_pattern(g, p, p->a, chunk_row, p->mask_index, p->max_row_nnz, kForward, (float *)ws);
   g.o0 = out; g.o0_row = out_row; g.o0_head = out_head;
   g.stats = stats;
-  const bool wide = piece_aligned(p, p->q, p->q_row, p->q_head) && piece_aligned(p, p->k, p->k_row, p->k_head) &&
-                    piece_aligned(p, p->v, p->v_row, p->v_head) && piece_aligned(p, out, out_row, out_head);
-  return launch(kForward, p->dtype, wide, g, as_stream(stream));
+  return launch(kForward, p->dtype, g, as_stream(stream));
 }
 
 extern "C" size_t gcnx_attention_backward_workspace_bytes(const gcnx_attention *p, int64_t t_max_row_nnz) {
@@ -773,7 +897,7 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
                GCNX_ERR_INVALID_ARG, "attention: null array in the transpose");
   GCNX_REQUIRE(!p->edge_mask || at->nnz == 0 || t_mask_index, GCNX_ERR_INVALID_ARG,
                "attention: the mask needs its index in the transpose");
-  GCNX_REQUIRE(p->a->n_rows == 0 || (out && dout && stats && out_row >= 0 && out_head >= 0 && dout_row >= 0 && dout_head >= 0),
+  GCNX_REQUIRE(p->a->n_rows == 0 || (out && dout && stats && stride_ok(out_row) && stride_ok(out_head) && stride_ok(dout_row) && stride_ok(dout_head)),
                GCNX_ERR_INVALID_ARG, "attention: bad output or gradient of it");
   GCNX_REQUIRE((dk == nullptr) == (dv == nullptr) && (dq || dk || (p->a->n_rows == 0 && p->a->n_cols == 0)),
                GCNX_ERR_INVALID_ARG, "attention: dq, or dk and dv, or all three");
@@ -784,23 +908,20 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
                    (!rows_are_cut(p->a->nnz, t_max_row_nnz) || t_chunk_row), GCNX_ERR_INVALID_ARG,
                "attention: chunk table needed");
   const int64_t hd = (int64_t)p->n_heads * p->head_dim, kd = (int64_t)p->n_kv_heads * p->head_dim;
-  const bool reads = piece_aligned(p, p->q, p->q_row, p->q_head) && piece_aligned(p, p->k, p->k_row, p->k_head) &&
-                     piece_aligned(p, p->v, p->v_row, p->v_head) && piece_aligned(p, dout, dout_row, dout_head);
   AttnArgs g = common_args(p);
   g.out = out; g.out_row = out_row; g.out_head = out_head;
   g.dout = dout; g.dout_row = dout_row; g.dout_head = dout_head;
+  g.dout_bytes = (uint32_t)(dout_row * (p->dtype == GCNX_F32 ? 4 : 2));
+  g.dout_head_bytes = (uint32_t)(dout_head * (p->dtype == GCNX_F32 ? 4 : 2));
   g.stats = const_cast<float *>(stats);
   g.stats4 = (f32x4 *)ws;
   float *part = (float *)((char *)ws + stats4_bytes(p));
   set_pattern(g, p, p->a, chunk_row, p->mask_index, p->max_row_nnz, kBackwardRows, part);
   g.o0 = dq; g.o0_row = hd; g.o0_head = p->head_dim;
-  if (int rc = launch(kBackwardRows, p->dtype, reads && piece_aligned(p, out, out_row, out_head) &&
-                                                   piece_aligned(p, dq, hd, p->head_dim), g, as_stream(stream)))
-    return rc;
+  if (int rc = launch(kBackwardRows, p->dtype, g, as_stream(stream))) return rc;
   if (!dk) return GCNX_OK;
   set_pattern(g, p, at, t_chunk_row, t_mask_index, t_max_row_nnz, kBackwardColumns, part);
   g.o0 = dk; g.o0_row = kd; g.o0_head = p->head_dim;
   g.o1 = dv; g.o1_row = kd; g.o1_head = p->head_dim;
-  return launch(kBackwardColumns, p->dtype, reads && piece_aligned(p, dk, kd, p->head_dim) && piece_aligned(p, dv, kd, p->head_dim),
-                g, as_stream(stream));
+  return launch(kBackwardColumns, p->dtype, g, as_stream(stream));
 }

@@ -23,6 +23,8 @@ ERR_UNSUPPORTED = -5
 ERR_COMM = -6
 COMM_ID_BYTES = 128
 F32, BF16, F16 = 0, 1, 2               # gcnx_dtype
+ADAMW_BLOCK = 256                      # GCNX_ADAMW_BLOCK
+ADAMW_WORKSPACE_BYTES = 256            # GCNX_ADAMW_WORKSPACE_BYTES
 
 
 class GcnxError(RuntimeError):
@@ -60,10 +62,34 @@ class AttentionStruct(C.Structure):
                 ("v", C.c_void_p), ("v_row", C.c_int64), ("v_head", C.c_int64)]
 
 
+class NormResidualStruct(C.Structure):
+    """Mirror of ``struct gcnx_norm_residual``."""
+    _fields_ = [("n", C.c_int64), ("dim", C.c_int32), ("dtype", C.c_int32), ("layer", C.c_int32), ("eps", C.c_float),
+                ("x", C.c_void_p), ("x_ld", C.c_int64), ("z", C.c_void_p), ("z_ld", C.c_int64),
+                ("gate", C.c_void_p), ("gate_ld", C.c_int64),
+                ("post_weight", C.c_void_p), ("res_scale", C.c_void_p), ("pre_weight", C.c_void_p)]
+
+
+class AdamWTensorStruct(C.Structure):
+    """Mirror of ``struct gcnx_adamw_tensor``."""
+    _fields_ = [("w", C.c_void_p), ("grad", C.c_void_p), ("n", C.c_int64), ("state", C.c_int64),
+                ("weight_decay", C.c_double)]
+
+
+class AdamWStruct(C.Structure):
+    """Mirror of ``struct gcnx_adamw``."""
+    _fields_ = [("w_dtype", C.c_int32), ("g_dtype", C.c_int32), ("state_bits", C.c_int32),
+                ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p),
+                ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("t", C.c_int64), ("t_dev", C.c_void_p), ("seed", C.c_uint64)]
+
+
 _i32, _i64, _u64, _f32, _f64 = C.c_int32, C.c_int64, C.c_uint64, C.c_float, C.c_double
 _p, _sz, _int = C.c_void_p, C.c_size_t, C.c_int
 _csr_p = C.POINTER(CsrStruct)
 _att_p = C.POINTER(AttentionStruct)
+_nrm_p = C.POINTER(NormResidualStruct)
 
 # name -> (restype, argtypes); must list every function include/gcnx.h declares.
 SIGNATURES = {
@@ -136,6 +162,10 @@ SIGNATURES = {
     "gcnx_attention_backward_workspace_bytes": (_sz, [_att_p, _i64]),
     "gcnx_attention_backward": (_int, [_att_p, _p, _csr_p, _p, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p,
                                        _p, _p, _sz, _p]),
+    "gcnx_norm_residual_forward": (_int, [_nrm_p, _p, _i64, _p, _i64, _p, _p]),
+    "gcnx_norm_residual_backward_workspace_bytes": (_sz, [_nrm_p]),
+    "gcnx_norm_residual_backward": (_int, [_nrm_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "gcnx_adamw_step": (_int, [C.POINTER(AdamWStruct), _i64, C.POINTER(AdamWTensorStruct), _p, _sz, _p]),
     "gcnx_xent_workspace_bytes": (_sz, [_i64]),
     "gcnx_masked_softmax_xent_f32": (_int, [_i64, _i32, _p, _i64, _p, _i64, _p, _f64, _p, _p, _i64,
                                             _p, _sz, _p]),

@@ -18,58 +18,9 @@
 // m and r are kept instead of the one number m - log r: at logits of 10^4, or a row
 // whose every value is the type's lowest, fp32 has no digits left for log r.
 #include "gcnx_common.h"
+#include "gcnx_piece.h"
 
 namespace gcnx {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-// A lane's piece of one head's vector: 16 bytes.  A head is spread over LPH lanes;
-// where the head is no multiple of the piece, the last piece overlaps the one
-// before it instead of reaching over the head's end: a lane multiplies its elements
-// `skip`.. only, and writes the others with the same values as their owner.  LPH 0:
-// heads shorter than a piece, one lane each, read element by element.
-template <typename T> struct Piece;
-template <> struct Piece<float> { typedef f32x4 raw; static constexpr int N = 4; };
-template <> struct Piece<__bf16> { typedef bf16x8 raw; static constexpr int N = 8; };
-template <> struct Piece<_Float16> { typedef f16x8 raw; static constexpr int N = 8; };
-
-// Addresses are kept as numbers and turned into pointers to global memory where
-// they are read: base + column * stride is one 32 x 32 + 64 bit multiply-add, and a
-// choice between two addresses does not become a generic (flat) access.
-typedef uint64_t Address;
-#define GCNX_GLOBAL __attribute__((address_space(1)))
-template <typename V>
-__device__ __forceinline__ V load_at(Address a) {
-  return *(const GCNX_GLOBAL V *)a;
-}
-__device__ __forceinline__ Address row_at(Address base, int32_t row, uint32_t stride) {
-  return base + (uint64_t)(uint32_t)row * stride;
-}
-
-// What lanes without an edge read: loads are never conditional (a load under a
-// branch is waited for before the next one can be issued into its registers).
-__device__ const f32x4 g_zeros[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
-
-__device__ __forceinline__ Address at_or_zeros(Address a, bool on) { return on ? a : (Address)&g_zeros[0]; }
-
-// One piece.  Rows need only their elements' alignment: global loads of 16 bytes
-// take any address.  NARROW: `dim` < a piece, the rest repeats the last element.
-template <typename T, bool NARROW>
-__device__ __forceinline__ typename Piece<T>::raw load_piece(Address a, int dim) {
-  typedef typename Piece<T>::raw raw;
-  typedef raw anywhere __attribute__((aligned(sizeof(T))));
-  if constexpr (!NARROW) {
-    return load_at<anywhere>(a);
-  } else {
-    raw x;
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i) x[i] = load_at<T>(a + sizeof(T) * (i < dim ? i : dim - 1));
-    return x;
-  }
-}
 
 // <a, b> + c over a piece.  16 bits: two exact products and their sum an instruction.
 template <typename T>
@@ -90,38 +41,6 @@ __device__ __forceinline__ float dot_piece(const typename Piece<T>::raw &a, cons
   return d;
 }
 
-template <typename T, bool NARROW>
-__device__ __forceinline__ void store_piece(T *p, int dim, const float (&v)[Piece<T>::N]) {
-  if constexpr (!NARROW) {
-    typename Piece<T>::raw x;
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i) x[i] = (T)v[i];
-    __builtin_memcpy(p, &x, sizeof(x));
-  } else {
-#pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i)
-      if (i < dim) p[i] = (T)v[i];
-  }
-}
-
-// Sum over groups of G neighbouring lanes, the result in every lane of the group.
-// Steps 1..8 are moves on the vector ALU: quad permutes, then the mirrors of 8 and
-// 16 lanes (every lane of a sub-group already holds the sub-group's sum).
-template <int G>
-__device__ __forceinline__ float group_sum(float v) {
-#define GCNX_DPP(ctrl) __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), ctrl, 0xF, 0xF, true))
-  if constexpr (G >= 2) v += GCNX_DPP(0xB1);
-  if constexpr (G >= 4) v += GCNX_DPP(0x4E);
-  if constexpr (G >= 8) v += GCNX_DPP(0x141);
-  if constexpr (G >= 16) v += GCNX_DPP(0x140);
-  if constexpr (G >= 32) v += __shfl_xor(v, 16, kWave);
-  if constexpr (G >= 64) v += __shfl_xor(v, 32, kWave);
-#undef GCNX_DPP
-  return v;
-}
-
-constexpr float kLog2e = 1.4426950408889634f;
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ bool is_lowest(float x) { return x == -__builtin_inff(); }
 
 constexpr int kUnroll = 4;   // edges in flight per lane
@@ -276,12 +195,6 @@ __device__ __forceinline__ typename Piece<T>::raw load_own(const AttnArgs &p, co
   return x;
 }
 
-// Nothing moves across: what is read ahead stays ahead of the sums.
-__device__ __forceinline__ void read_ahead_fence() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 // Joins two softmax states (m, l, acc); m = -inf: nothing summed yet.
 template <int N>
 __device__ __forceinline__ void join(float &m, float &l, float (&acc)[N], float m2, float l2, const float (&acc2)[N]) {
@@ -307,7 +220,8 @@ __device__ __forceinline__ void finish_forward(const AttnArgs &p, const Task &t,
   }
 }
 
-// Elements of a partial vector of one head in the workspace.
+// Elements of a partial vector of one head in the workspace: the vector (two in the
+// backward passes), then four numbers, of which two (one) are used.
 template <typename T, int LPH>
 constexpr int kPartWide = (LPH ? LPH : 1) * Piece<T>::N;
 
@@ -370,85 +284,102 @@ __global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
   }
   if (t.edge != 0 || !t.live) return;
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (kPartWide<T, LPH> + 2);
-#pragma unroll
-    for (int i = 0; i < N; ++i) part[2 + t.d0 + i] = acc[i];
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (kPartWide<T, LPH> + 4);
+    store_floats<N>(part + t.d0, acc);
     if (t.d0 == 0) {
-      part[0] = m;
-      part[1] = l;
+      part[kPartWide<T, LPH>] = m;
+      part[kPartWide<T, LPH> + 1] = l;
     }
     return;
   }
   finish_forward<T, LPH, N>(p, t, m, l, acc);
 }
 
-// Joining the pieces of cut rows.  A workgroup per chunk and head tile, at work if a
-// cut row begins in the chunk: its pieces are slot 1 of that chunk and slot 0 of the
-// chunks after it.  They are dealt to the lane groups, each joins its own in order,
-// then the groups are joined through LDS in order: a fixed tree.
+// Joining the pieces of cut rows: those that begin in one of kJoinChunks chunks, a
+// tile of heads of them, by a workgroup.  A row's pieces are slot 1 of the chunk that
+// it begins in and slot 0 of the chunks after it; they are dealt to groups of lanes, kJoinAhead read at a time, each group joins its own in order, then groups
+// are joined by exchanges in the wavefront and through LDS: a fixed tree.
+constexpr int kJoinChunks = 4;
+constexpr int kJoinAhead = 4;
+
 struct JoinTask {
-  int64_t first, last;
-  int32_t group, groups, per_wave, heads_log2;
+  int64_t first, last;          // chunks of the row
   __device__ __forceinline__ const float *part(const AttnArgs &p, int64_t c) const {
-    return p.part + (c * 2 + (c == first)) * p.part_floats;
-  }
-  template <int L>
-  __device__ __forceinline__ int thread_of(int g) const {   // the thread of group g with this lane's head and piece
-    const int lane = threadIdx.x & (kWave - 1), low = lane & ((L << heads_log2) - 1);
-    return (g / per_wave) * kWave + (g % per_wave) * (L << heads_log2) + low;
+    return p.part + ((c <= last ? c : last) * 2 + (c == first)) * p.part_floats;
   }
 };
 
-template <typename T, int LPH>
-__device__ __forceinline__ bool find_join(const AttnArgs &p, int heads, Task &t, JoinTask &j) {
-  constexpr int L = LPH ? LPH : 1;
-  j.first = blockIdx.x;
-  const int64_t first = j.first * p.segment, next = first + p.segment;
-  if (next >= p.nnz) return false;
-  t.row = p.chunk_row[next / kChunkUnit];
-  const int64_t beg = p.row_ptr[t.row], end = p.row_ptr[t.row + 1];
-  if (beg < first || beg >= next || end - beg <= p.segment) return false;
-  j.last = (end - 1) / p.segment;
-  int slot;
-  place_lane<T, LPH>(p, heads, blockIdx.y, t, slot);
-  j.heads_log2 = p.heads_log2;
-  j.per_wave = (kWave / L) >> p.heads_log2;
-  j.groups = j.per_wave * kWavesPerBlock;
-  j.group = slot + j.per_wave * (threadIdx.x >> 6);
-  return true;
+// Which of the workgroup's chunks have a cut row begin in them, a lane a chunk; row
+// and last chunk of the lane's.
+__device__ __forceinline__ uint64_t find_joins(const AttnArgs &p, int64_t &row, int64_t &last) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t first = ((int64_t)blockIdx.x * kJoinChunks + lane) * p.segment, next = first + p.segment;
+  bool found = false;
+  row = last = 0;
+  if (lane < kJoinChunks && next < p.nnz) {
+    row = p.chunk_row[next / kChunkUnit];
+    const int64_t beg = p.row_ptr[row], end = p.row_ptr[row + 1];
+    last = (end - 1) / p.segment;
+    found = beg >= first && beg < next && end - beg > p.segment;
+  }
+  return __ballot(found);
 }
 
 template <typename T, int LPH>
 __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs p) {
-  constexpr int N = Piece<T>::N;
-  __shared__ float sh[kBlock][N + 2];
+  constexpr int N = Piece<T>::N, L = LPH ? LPH : 1;
+  const int span = L << p.heads_log2, groups = kBlock / span;     // lanes of a group
+  __shared__ float sh[kWavesPerBlock][kWave][N + 2];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   Task t;
   JoinTask j;
-  if (!find_join<T, LPH>(p, p.heads, t, j)) return;
-  float m = -__builtin_inff(), l = 0.0f, acc[N] = {};
-  if (t.live)
-    for (int64_t c = j.first + j.group; c <= j.last; c += j.groups) {
-      const float *part = j.part(p, c) + (int64_t)t.head * (kPartWide<T, LPH> + 2);
-      float a2[N];
+  int slot;
+  place_lane<T, LPH>(p, p.heads, blockIdx.y, t, slot);
+  int64_t rows, lasts;
+  for (uint64_t left = find_joins(p, rows, lasts); left; left &= left - 1) {
+    const int chunk = __builtin_ctzll(left);
+    t.row = __shfl(rows, chunk, kWave);
+    j.first = (int64_t)blockIdx.x * kJoinChunks + chunk;
+    j.last = __shfl(lasts, chunk, kWave);
+    float m = -__builtin_inff(), l = 0.0f, acc[N] = {};
+    for (int64_t c = j.first + threadIdx.x / span; c <= j.last; c += kJoinAhead * groups) {
+      float m2[kJoinAhead], l2[kJoinAhead], a2[kJoinAhead][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) a2[i] = part[2 + t.d0 + i];
-      join<N>(m, l, acc, part[0], part[1], a2);
+      for (int u = 0; u < kJoinAhead; ++u) {
+        const float *part = j.part(p, c + u * groups) + (int64_t)t.head * (kPartWide<T, LPH> + 4);
+        m2[u] = part[kPartWide<T, LPH>];
+        l2[u] = part[kPartWide<T, LPH> + 1];
+        load_floats<N>(part + t.d0, a2[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinAhead; ++u)
+        if (c + u * groups <= j.last) join<N>(m, l, acc, m2[u], l2[u], a2[u]);
     }
-  float *mine = sh[threadIdx.x];
-  mine[0] = m;
-  mine[1] = l;
+    for (int off = span; off < kWave; off <<= 1) {
+      float m2 = __shfl_xor(m, off, kWave), l2 = __shfl_xor(l, off, kWave), a2[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) mine[2 + i] = acc[i];
-  __syncthreads();
-  if (j.group != 0 || !t.live) return;
-  for (int g = 1; g < j.groups; ++g) {
-    const float *other = sh[j.thread_of<LPH ? LPH : 1>(g)];
-    float a2[N];
+      for (int i = 0; i < N; ++i) a2[i] = __shfl_xor(acc[i], off, kWave);
+      join<N>(m, l, acc, m2, l2, a2);
+    }
+    __syncthreads();
+    if (lane < span) {
+      sh[wave][lane][0] = m;
+      sh[wave][lane][1] = l;
 #pragma unroll
-    for (int i = 0; i < N; ++i) a2[i] = other[2 + i];
-    join<N>(m, l, acc, other[0], other[1], a2);
+      for (int i = 0; i < N; ++i) sh[wave][lane][2 + i] = acc[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < span && t.live) {
+#pragma unroll
+      for (int w = 1; w < kWavesPerBlock; ++w) {
+        float a2[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) a2[i] = sh[w][lane][2 + i];
+        join<N>(m, l, acc, sh[w][lane][0], sh[w][lane][1], a2);
+      }
+      finish_forward<T, LPH, N>(p, t, m, l, acc);
+    }
   }
-  finish_forward<T, LPH, N>(p, t, m, l, acc);
 }
 
 // Row pass of the backward: delta, dq.  Writes m, r, delta side by side for the
@@ -540,12 +471,9 @@ __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArg
   if (t.edge != 0 || !t.live) return;
   if (r == 0.0f) d0 = rest = 0.0f;   // a row of zeros hands nothing on, whatever its gradient holds
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 1);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      part[t.d0 + i] = acc[i];
-      part[kPartWide<T, LPH> + t.d0 + i] = low[i];
-    }
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 4);
+    store_floats<N>(part + t.d0, acc);
+    store_floats<N>(part + kPartWide<T, LPH> + t.d0, low);
     if (t.d0 == 0) part[2 * kPartWide<T, LPH>] = rest;
     return;
   }
@@ -627,12 +555,9 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
   }
   if (t.edge != 0 || !t.live) return;
   if (t.piece >= 0) {
-    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 1);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      part[t.d0 + i] = dk[i];
-      part[kPartWide<T, LPH> + t.d0 + i] = dv[i];
-    }
+    float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 4);
+    store_floats<N>(part + t.d0, dk);
+    store_floats<N>(part + kPartWide<T, LPH> + t.d0, dv);
     return;
   }
 #pragma unroll
@@ -645,60 +570,86 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
 // head (A, B and rest of the row pass; dk, dv and nothing of the column pass).
 template <typename T, int LPH, bool COLUMNS>
 __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArgs p) {
-  constexpr int N = Piece<T>::N;
-  __shared__ float sh[kBlock][2 * N + 1];
+  constexpr int N = Piece<T>::N, L = LPH ? LPH : 1;
+  const int span = L << p.heads_log2, groups = kBlock / span;     // lanes of a group
+  __shared__ float sh[kWavesPerBlock][kWave][2 * N + 1];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   Task t;
   JoinTask j;
-  if (!find_join<T, LPH>(p, COLUMNS ? p.kv_heads : p.heads, t, j)) return;
-  float a[N] = {}, b[N] = {}, rest = 0.0f;
-  if (t.live)
-    for (int64_t c = j.first + j.group; c <= j.last; c += j.groups) {
-      const float *part = j.part(p, c) + (int64_t)t.head * (2 * kPartWide<T, LPH> + 1);
+  int slot;
+  place_lane<T, LPH>(p, COLUMNS ? p.kv_heads : p.heads, blockIdx.y, t, slot);
+  int64_t rows, lasts;
+  for (uint64_t left = find_joins(p, rows, lasts); left; left &= left - 1) {
+    const int chunk = __builtin_ctzll(left);
+    t.row = __shfl(rows, chunk, kWave);
+    j.first = (int64_t)blockIdx.x * kJoinChunks + chunk;
+    j.last = __shfl(lasts, chunk, kWave);
+    float a[N] = {}, b[N] = {}, rest = 0.0f;
+    for (int64_t c = j.first + threadIdx.x / span; c <= j.last; c += kJoinAhead * groups) {
+      float a2[kJoinAhead][N], b2[kJoinAhead][N], rest2[kJoinAhead];
+#pragma unroll
+      for (int u = 0; u < kJoinAhead; ++u) {
+        const float *part = j.part(p, c + u * groups) + (int64_t)t.head * (2 * kPartWide<T, LPH> + 4);
+        load_floats<N>(part + t.d0, a2[u]);
+        load_floats<N>(part + kPartWide<T, LPH> + t.d0, b2[u]);
+        rest2[u] = COLUMNS ? 0.0f : part[2 * kPartWide<T, LPH>];
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinAhead; ++u)
+        if (c + u * groups <= j.last) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            a[i] += a2[u][i];
+            b[i] += b2[u][i];
+          }
+          rest += rest2[u];
+        }
+    }
+    for (int off = span; off < kWave; off <<= 1) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        a[i] += part[t.d0 + i];
-        b[i] += part[kPartWide<T, LPH> + t.d0 + i];
+        a[i] += __shfl_xor(a[i], off, kWave);
+        b[i] += __shfl_xor(b[i], off, kWave);
       }
-      if (!COLUMNS) rest += part[2 * kPartWide<T, LPH>];
+      rest += __shfl_xor(rest, off, kWave);
     }
+    __syncthreads();
+    if (lane < span) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    sh[threadIdx.x][i] = a[i];
-    sh[threadIdx.x][N + i] = b[i];
-  }
-  sh[threadIdx.x][2 * N] = rest;
-  float m = 0.0f, r = 0.0f, d0 = 0.0f;
-  if (!COLUMNS && j.group == 0) load_row<T, LPH>(p, t, m, r, d0);
-  __syncthreads();
-  if (j.group != 0 || !t.live) return;
-  for (int o = 1; o < j.groups; ++o) {
-    const float *other = sh[j.thread_of<LPH ? LPH : 1>(o)];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      a[i] += other[i];
-      b[i] += other[N + i];
+      for (int i = 0; i < N; ++i) {
+        sh[wave][lane][i] = a[i];
+        sh[wave][lane][N + i] = b[i];
+      }
+      sh[wave][lane][2 * N] = rest;
     }
-    rest += other[2 * N];
-  }
-  if constexpr (COLUMNS) {
+    float m = 0.0f, r = 0.0f, d0 = 0.0f;
+    if (!COLUMNS && wave == 0) load_row<T, LPH>(p, t, m, r, d0);
+    __syncthreads();
+    if (threadIdx.x < span && t.live) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] *= p.scale;
-    store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, a);
-    store_piece<T, LPH == 0>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, p.dim, b);
-  } else {
-    if (r == 0.0f) d0 = rest = 0.0f;
-    finish_rows<T, LPH, N>(p, t, m, r, d0, rest, a, b);
+      for (int w = 1; w < kWavesPerBlock; ++w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          a[i] += sh[w][lane][i];
+          b[i] += sh[w][lane][N + i];
+        }
+        rest += sh[w][lane][2 * N];
+      }
+      if constexpr (COLUMNS) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] *= p.scale;
+        store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, a);
+        store_piece<T, LPH == 0>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, p.dim, b);
+      } else {
+        if (r == 0.0f) d0 = rest = 0.0f;
+        finish_rows<T, LPH, N>(p, t, m, r, d0, rest, a, b);
+      }
+    }
   }
 }
 
 // ------------------------------------------------------------------ host side
 enum { kForward = 0, kBackwardRows = 1, kBackwardColumns = 2 };
-
-static int log2_ceil(int64_t x) {
-  int l = 0;
-  while (((int64_t)1 << l) < x) ++l;
-  return l;
-}
 
 static int piece_elements(int dtype) { return dtype == GCNX_F32 ? 4 : 8; }
 
@@ -711,17 +662,20 @@ static int lanes_per_head(int dtype, int dim) {
 static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim) {
   const int lph = lanes_per_head(dtype, dim);
   const int64_t wide = (int64_t)(lph ? lph : 1) * piece_elements(dtype);
-  return pass == kForward ? heads * (wide + 2) : (pass == kBackwardRows ? heads : kv_heads) * (2 * wide + 1);
+  return pass == kForward ? heads * (wide + 4) : (pass == kBackwardRows ? heads : kv_heads) * (2 * wide + 4);
 }
 
-// Edges a wavefront takes of one row at most.
-static int segment_of(int64_t nnz) {
-  (void)nnz;
-  return 512;
-}
+// Edges a wavefront takes of one row at most: a long row is the last to end where
+// there are few rows, and pieces cost partial results where there are many.
+// Forward and its join, us, at 64 / 128 / 256 / 512 (8 x 32 and 8 on 2 x 64 heads):
+// 0.1 M edges 29 / 35 / 49 / 81, 0.9 M 255 / 273 / 310 / 363, 1 M 125 / 121 / 121 / 139,
+// 8.5 M 1280 / 1225 / 1138 / 1085.
+static int segment_of(int64_t nnz) { return nnz <= (1 << 18) ? 64 : nnz <= (1 << 20) ? 128 : nnz <= (1 << 22) ? 256 : 512; }
 
+// The second launch costs what about three pieces do one after the other (5 us).
 static bool rows_are_cut(int64_t nnz, int64_t max_row_nnz) {
-  return nnz > segment_of(nnz) && (max_row_nnz <= 0 || max_row_nnz > segment_of(nnz) || nnz > 0x7fffffff);
+  const int64_t uncut = 4 * segment_of(nnz);
+  return nnz > uncut && (max_row_nnz <= 0 || max_row_nnz > uncut || nnz > 0x7fffffff);
 }
 
 static size_t part_bytes(const gcnx_attention *p, int64_t max_row_nnz, int pass) {
@@ -736,16 +690,16 @@ static size_t stats4_bytes(const gcnx_attention *p) {
 }
 
 template <typename T, int LPH, bool SHIFTS>
-static void launch_pass(int pass, const AttnArgs &p, dim3 grid, dim3 joins, hipStream_t stream) {
+static void launch_pass(int pass, const AttnArgs &p, dim3 grid, const AttnArgs &joined, dim3 joins, hipStream_t stream) {
   if (pass == kForward) {
     hipLaunchKernelGGL((attention_forward_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH>), joins, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH>), joins, dim3(kBlock), 0, stream, joined);
   } else if (pass == kBackwardRows) {
     hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, false>), joins, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, false>), joins, dim3(kBlock), 0, stream, joined);
   } else {
     hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, true>), joins, dim3(kBlock), 0, stream, p);
+    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, true>), joins, dim3(kBlock), 0, stream, joined);
   }
 }
 
@@ -756,10 +710,13 @@ static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   const int heads_log2 = log2_ceil(heads);
   p.heads_log2 = heads_log2 < slots_log2 ? heads_log2 : slots_log2;
   const int spare = slots_log2 - p.heads_log2;
-  // edges side by side: about kUnroll per lane at the average row; what is left
-  // takes further rows
+  // edges side by side, what is left takes further rows: as many edges as the average
+  // row has, so that rows end soon, unless there are rows enough to fill the machine
+  // (8 wavefronts a SIMD): then kUnroll edges a lane, so that few lanes idle.
+  // (Cora: 11 us against 18 with kUnroll; 2^18 rows of 2: 285 against 160.)
   const int64_t items = ceil_div(p.nnz * (pass == kBackwardColumns ? p.group : 1), p.n_rows);
-  const int e = log2_ceil(ceil_div(items, kUnroll));
+  int e = log2_ceil(items);
+  if ((p.n_rows << (e < spare ? e : spare)) >> spare > 8 * 1024) e = log2_ceil(ceil_div(items, kUnroll));
   p.edge_log2 = e < spare ? e : spare;
   p.row_log2 = spare - p.edge_log2;
   p.tiles = (int)ceil_div(heads, (int64_t)1 << p.heads_log2);
@@ -767,9 +724,13 @@ static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   int64_t blocks = ceil_div(p.n_pieces + ceil_div(p.n_rows, (int64_t)1 << p.row_log2), kWavesPerBlock);
   blocks = p.tiles_log2 >= 0 ? ceil_div(blocks, 8 >> p.tiles_log2) * 8 : blocks * p.tiles;
   GCNX_REQUIRE(blocks <= 0x7fffffff && p.n_pieces / 2 <= 0x7fffffff, GCNX_ERR_UNSUPPORTED, "attention: too many rows for one launch");
-  const dim3 grid((unsigned)blocks), joins((unsigned)(p.n_pieces / 2), (unsigned)p.tiles);
-  if (p.val || p.mask) launch_pass<T, LPH, true>(pass, p, grid, joins, stream);
-  else launch_pass<T, LPH, false>(pass, p, grid, joins, stream);
+  const dim3 grid((unsigned)blocks);
+  // few rows of many pieces: a workgroup per head instead of one for a tile of them
+  AttnArgs joined = p;
+  if (p.n_pieces / 2 / p.n_rows >= 16) joined.heads_log2 = 0;
+  const dim3 joins((unsigned)ceil_div(p.n_pieces / 2, kJoinChunks), (unsigned)ceil_div(heads, (int64_t)1 << joined.heads_log2));
+  if (p.val || p.mask) launch_pass<T, LPH, true>(pass, p, grid, joined, joins, stream);
+  else launch_pass<T, LPH, false>(pass, p, grid, joined, joins, stream);
   GCNX_CHECK_LAUNCH();
   return GCNX_OK;
 }

@@ -11,8 +11,10 @@ case and the ``part(k) - b2`` of the opt-in Clenshaw recurrence.  The large-grap
 engine (``gcn_amd/engine.py``) uses none of them.
 All functions raise on CPU tensors -- there is no fallback path.
 """
+import contextlib
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -474,7 +476,7 @@ def _check_heads(t, name, rows, dim=None, like=None):
         raise RuntimeError("%s must be a CUDA (ROCm) tensor; gcn_amd has no CPU path" % name)
     if t.dtype not in _DTYPES:
         raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1 and t.numel()):
         raise ValueError("%s must be [rows, heads, head_dim] with contiguous head vectors" % name)
     if t.shape[0] != rows:
         raise ValueError("%s has %d rows, the matrix asks for %d" % (name, t.shape[0], rows))
@@ -508,6 +510,14 @@ def _attention_struct(a, q, k, v, scale, use_values, mask):
         k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1))
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes ``device`` current for the launches of a ``with`` block."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _scratch(nbytes, device):
     # from torch's allocator, which orders the memory by stream and owns it in a
     # capture: two streams, or two recorded graphs, never share it
@@ -535,7 +545,7 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
         if out.shape[1] != q.shape[1] or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
             raise ValueError("out must be [n_rows, heads, head_dim] of distinct elements")
     stats = torch.empty((a.n_rows, q.shape[1], 2), dtype=torch.float32, device=q.device) if want_stats else None
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         ws = _scratch(lib.gcnx_attention_workspace_bytes(C.byref(p)), q.device)
         _lib.check(lib.gcnx_attention_forward(C.byref(p), _ptr(a.chunk_row), _ptr(out), out.stride(0), out.stride(1),
                                               _ptr(stats), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
@@ -564,7 +574,7 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
     dq = new(q) if need_q else None
     dk, dv = (new(k), new(v)) if need_kv else (None, None)
     midx = at.input_index if mask is not None else None
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         ws = _scratch(lib.gcnx_attention_backward_workspace_bytes(C.byref(p), at.max_row_nnz()), q.device)
         _lib.check(lib.gcnx_attention_backward(
             C.byref(p), _ptr(a.chunk_row), at.struct_ref(), _ptr(at.chunk_row), _ptr(midx), at.max_row_nnz(), _ptr(out),
@@ -598,6 +608,128 @@ class _AttentionFn(torch.autograd.Function):
 def attention_autograd(a, q, k, v, scale=None, use_values=False, mask=None):
     """:func:`attention` on the autograd tape."""
     return _AttentionFn.apply(q, k, v, a, scale, use_values, mask)
+
+
+# ----------------------------------------------------------------------- norms
+def _check_rows(t, name, like=None):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise RuntimeError("%s must be a CUDA (ROCm) tensor; gcn_amd has no CPU path" % name)
+    if t.dtype not in _DTYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1 and t.numel()):
+        raise ValueError("%s must be a row-major 2-D tensor" % name)
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError("%s differs from x in shape, dtype or device" % name)
+
+
+def _check_weight(w, name, x):
+    if w.dtype != torch.float32 or w.dim() != 1 or w.numel() != x.shape[1] or not w.is_contiguous() or w.device != x.device:
+        raise ValueError("%s must be contiguous float32 [%d] on x's device" % (name, x.shape[1]))
+
+
+def _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps):
+    _check_rows(x, "x")
+    if kind not in ("rms", "layer"):
+        raise ValueError("kind must be 'rms' or 'layer', got %r" % (kind,))
+    if not 1 <= x.shape[1] <= 4096:
+        raise ValueError("rows of 1..4096 elements, got %d" % x.shape[1])
+    if z is not None:
+        _check_rows(z, "z", x)
+    elif gate is not None or post_weight is not None or res_scale is not None:
+        raise ValueError("gate, post_weight and res_scale belong to z")
+    elif pre_weight is None:
+        raise ValueError("neither z nor pre_weight: nothing to do")
+    if gate is not None:
+        _check_rows(gate, "gate", x)
+    for w, name in ((post_weight, "post_weight"), (res_scale, "res_scale"), (pre_weight, "pre_weight")):
+        if w is not None:
+            _check_weight(w, name, x)
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    ld = lambda t: t.stride(0) if t is not None else 0
+    return _lib.NormResidualStruct(x.shape[0], x.shape[1], _DTYPES[x.dtype], int(kind == "layer"), float(eps), x.data_ptr(),
+                                   x.stride(0), ptr(z), ld(z), ptr(gate), ld(gate), ptr(post_weight), ptr(res_scale),
+                                   ptr(pre_weight))
+
+
+def norm_residual(x, z=None, gate=None, post_weight=None, res_scale=None, pre_weight=None, kind="rms", eps=1e-6,
+                  want_stats=False):
+    """``(y, h, stats)``: the end of one block of a deep network and the norm in front
+    of the next, row by row in one pass:
+    ``y = x + res_scale * sigmoid(gate) * (norm(z) * post_weight)``,
+    ``h = norm(y) * pre_weight``.  ``x`` (the residual stream), ``z`` (the block's
+    output) and ``gate`` (logits) are row-major [n, dim], dim up to 4096, one of
+    float32, bfloat16 and float16; the weights float32 [dim].  What is None is left
+    out: no ``gate`` or ``res_scale`` multiplies by one, no ``post_weight`` takes ``z``
+    as it is, no ``pre_weight`` gives no ``h`` (None), no ``z`` gives ``y = x`` (``x``
+    itself) and ``h = norm(x) * pre_weight``.  ``norm`` divides by the root mean square
+    (``kind="rms"``) or takes the mean off first (``"layer"``).  ``stats`` (None unless
+    ``want_stats``) is what :func:`norm_residual_bwd` needs."""
+    lib = _lib.load()
+    p = _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps)
+    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = new() if z is not None else x
+    h = new() if pre_weight is not None else None
+    stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device) if want_stats else None
+    if x.shape[0]:
+        with _on(x.device):
+            _lib.check(lib.gcnx_norm_residual_forward(C.byref(p), _ptr(y), y.stride(0), _ptr(h), x.shape[1], _ptr(stats), _stream()))
+    return y, h, stats
+
+
+def norm_residual_bwd(x, dy, dh, stats, z=None, gate=None, post_weight=None, res_scale=None, pre_weight=None, kind="rms",
+                      eps=1e-6):
+    """``(dx, dz, dgate, dpost, dres, dpre)`` of :func:`norm_residual` for the gradients
+    ``dy`` and ``dh`` of its outputs (None: zero); None where there is no such operand.
+    The row gradients have the type of ``x``, those of the weights are float32, summed
+    over the rows in a fixed order."""
+    lib = _lib.load()
+    p = _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps)
+    for t, name in ((dy, "dy"), (dh, "dh")):
+        if t is not None:
+            _check_rows(t, name, x)
+    if dh is not None and pre_weight is None:
+        raise ValueError("dh without pre_weight")
+    n, dim = x.shape
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (n, 4) or not stats.is_contiguous() or stats.device != x.device:
+        raise ValueError("stats must be what norm_residual(..., want_stats=True) returned")
+    new = lambda on: torch.empty((n, dim), dtype=x.dtype, device=x.device) if on else None
+    dx, dz, dgate = new(True), new(z is not None), new(gate is not None)
+    sums = [w is not None for w in (post_weight, res_scale, pre_weight)]
+    rows = n > 0 and (sums[0] or sums[1] or dh is not None)
+    # no rows, or no gradient behind pre_weight: a sum over nothing
+    made = [(torch.empty if rows and (i < 2 or dh is not None) else torch.zeros)(dim, dtype=torch.float32, device=x.device)
+            if on else None for i, on in enumerate(sums)]
+    dpost, dres, dpre = made
+    if n:
+        with _on(x.device):
+            ws = _scratch(lib.gcnx_norm_residual_backward_workspace_bytes(C.byref(p)) if rows else 0, x.device)
+            _lib.check(lib.gcnx_norm_residual_backward(
+                C.byref(p), _ptr(dy), dy.stride(0) if dy is not None else 0, _ptr(dh), dh.stride(0) if dh is not None else 0,
+                _ptr(stats), _ptr(dx), _ptr(dz), _ptr(dgate), _ptr(dpost), _ptr(dres), _ptr(dpre if dh is not None else None),
+                _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+    return dx, dz, dgate, dpost, dres, dpre
+
+
+class _NormResidualFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, z, gate, post_weight, res_scale, pre_weight, kind, eps):
+        y, h, stats = norm_residual(x, z, gate, post_weight, res_scale, pre_weight, kind, eps, want_stats=True)
+        ctx.save_for_backward(x, z, gate, post_weight, res_scale, pre_weight, stats)
+        ctx.how = (kind, eps)
+        ctx.set_materialize_grads(False)
+        return y if z is not None else x.view_as(x), h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        x, z, gate, post_weight, res_scale, pre_weight, stats = ctx.saved_tensors
+        rows = lambda t: t if t is None or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+        return norm_residual_bwd(x, rows(dy), rows(dh), stats, z, gate, post_weight, res_scale, pre_weight, *ctx.how) + (None, None)
+
+
+def norm_residual_autograd(x, z=None, gate=None, post_weight=None, res_scale=None, pre_weight=None, kind="rms", eps=1e-6):
+    """``(y, h)`` of :func:`norm_residual` on the autograd tape."""
+    return _NormResidualFn.apply(x, z, gate, post_weight, res_scale, pre_weight, kind, eps)
 
 
 # ------------------------------------------------------------- loss / accuracy
@@ -863,6 +995,118 @@ def adam_step(w, grad, m, v, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, weight_dec
     return w
 
 
+class AdamWState(object):
+    """The moments of :func:`adamw_step` for a list of tensors (:func:`adamw_state`),
+    all in two flat buffers: tensor i's are the elements from ``offsets[i]`` on, every
+    offset a multiple of 256.  ``bits`` 32: ``exp_avg`` and ``exp_avg_sq`` float32.  8:
+    float8_e4m3fn codes, ``exp_avg`` of m and ``exp_avg_sq`` of sqrt(v), each to be
+    multiplied by its block of 256's power of two in ``exp_avg_scale`` /
+    ``exp_avg_sq_scale``; ``seed`` keys the random rounding."""
+
+    def __init__(self, params, bits, seed):
+        self.bits, self.seed = bits, int(seed) & (2 ** 64 - 1)
+        self.sizes = [p.numel() for p in params]
+        self.dtype, self.device = params[0].dtype, params[0].device
+        self.offsets, total = [], 0
+        for n in self.sizes:
+            self.offsets.append(total)
+            total += -(-n // _lib.ADAMW_BLOCK) * _lib.ADAMW_BLOCK
+        zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=self.device)
+        if bits == 32:
+            self.exp_avg, self.exp_avg_sq = zeros(total, torch.float32), zeros(total, torch.float32)
+            self.exp_avg_scale = self.exp_avg_sq_scale = None
+        else:
+            self.exp_avg, self.exp_avg_sq = [zeros(total, torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)]
+            self.exp_avg_scale, self.exp_avg_sq_scale = [torch.ones_like(zeros(total // _lib.ADAMW_BLOCK, torch.float32))
+                                                         for _ in range(2)]
+        self._table = np.zeros(len(self.sizes), dtype=[("w", "u8"), ("grad", "u8"), ("n", "i8"), ("state", "i8"), ("decay", "f8")])
+        self._table["state"] = self.offsets
+
+    def moments(self, i):
+        """``(m, v)`` of tensor i as flat float32 tensors."""
+        at, n = self.offsets[i], self.sizes[i]
+        m, v = self.exp_avg[at:at + n].float(), self.exp_avg_sq[at:at + n].float()
+        if self.bits == 8:
+            block = torch.arange(at, at + n, device=self.device) // _lib.ADAMW_BLOCK
+            m, v = m * self.exp_avg_scale[block], (v * self.exp_avg_sq_scale[block]) ** 2
+        return m, v
+
+
+def adamw_state(params, bits=32, seed=0):
+    """A zero :class:`AdamWState` for a list of contiguous tensors of one dtype
+    (float32, bfloat16 or float16) on one device; ``bits`` 32 or 8."""
+    params = list(params)
+    if not params:
+        raise ValueError("no tensors")
+    if bits not in (32, 8):
+        raise ValueError("bits must be 32 or 8, got %r" % (bits,))
+    for p in params:
+        if not isinstance(p, torch.Tensor) or p.device.type != "cuda":
+            raise RuntimeError("params must be CUDA (ROCm) tensors; gcn_amd has no CPU path")
+        if p.dtype not in _DTYPES:
+            raise TypeError("params must be float32, bfloat16 or float16, got %s" % (p.dtype,))
+        if p.dtype != params[0].dtype or p.device != params[0].device:
+            raise ValueError("params differ in dtype or device")
+    return AdamWState(params, bits, seed)
+
+
+def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01):
+    """One in-place AdamW update of every tensor of ``params`` in one launch (one per 64
+    tensors): ``m = beta1 m + (1 - beta1) g``, ``v = beta2 v + (1 - beta2) g^2``,
+    ``w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)``.
+    ``state`` is the list's :func:`adamw_state`; ``grads`` (one dtype: float32, bfloat16
+    or float16) has one contiguous tensor a param, or None: that param and its state
+    stay as they are.  ``t`` counts from 1 and is either a Python int or a device counter
+    (read when the kernels run); ``weight_decay`` is a number or one a param.  The
+    decoupled many-tensor sibling of :func:`adam_step`."""
+    lib = _lib.load()
+    count = len(state.sizes)
+    params, grads = list(params), list(grads)
+    if len(params) != count or len(grads) != count:
+        raise ValueError("%d params and %d grads for a state of %d tensors" % (len(params), len(grads), count))
+    dtype, dev, g_dtype = state.dtype, state.device, None
+    w_ptr, g_ptr, sizes = [], [], []
+    for p, g, n in zip(params, grads, state.sizes):
+        if p.dtype != dtype or p.device != dev or p.numel() != n or not p.is_contiguous():
+            raise ValueError("params must be the contiguous tensors the state was made for")
+        if g is None:
+            w_ptr.append(p.data_ptr())
+            g_ptr.append(0)
+            sizes.append(0)
+            continue
+        if g_dtype is None:
+            g_dtype = g.dtype
+            if g_dtype not in _DTYPES:
+                raise TypeError("grads must be float32, bfloat16 or float16, got %s" % (g_dtype,))
+        if g.dtype != g_dtype or g.device != dev or g.numel() != n or not g.is_contiguous():
+            raise ValueError("grads must be contiguous, of one dtype, on the params' device and of their sizes")
+        w_ptr.append(p.data_ptr())
+        g_ptr.append(g.data_ptr())
+        sizes.append(n)
+    live = [w for w, n in zip(w_ptr, sizes) if n]
+    if len(set(live)) != len(live):
+        raise ValueError("a tensor is twice among the params")
+    if not live:
+        return params
+    if isinstance(t, torch.Tensor):
+        if t.device != dev or t.dtype != torch.int64 or t.numel() != 1:
+            raise ValueError("t must be an int or a one-element int64 tensor on the params' device")
+        t_ptr, t_host = t.data_ptr(), 0
+    else:
+        t_ptr, t_host = None, int(t)
+    table = state._table.copy()
+    table["w"], table["grad"], table["n"], table["decay"] = w_ptr, g_ptr, sizes, weight_decay
+    ptr = lambda x: x.data_ptr() if x is not None else None
+    p = _lib.AdamWStruct(_DTYPES[dtype], _DTYPES[g_dtype], state.bits, ptr(state.exp_avg), ptr(state.exp_avg_sq),
+                         ptr(state.exp_avg_scale), ptr(state.exp_avg_sq_scale), float(lr), float(beta1), float(beta2), float(eps),
+                         t_host, t_ptr, state.seed)
+    with _on(dev):
+        ws = _scratch(_lib.ADAMW_WORKSPACE_BYTES if t_ptr else 0, dev)
+        _lib.check(lib.gcnx_adamw_step(C.byref(p), count, table.ctypes.data_as(C.POINTER(_lib.AdamWTensorStruct)), _ptr(ws),
+                                       ws.numel() if ws is not None else 0, _stream()))
+    return params
+
+
 def l2_loss(w, scale=1.0, add=None):
     """One-element tensor ``(add or 0) + scale * sum(w ** 2) / 2`` (reference
     gcn/models.py:148-149: ``weight_decay * tf.nn.l2_loss(var)`` added into the
@@ -896,4 +1140,6 @@ def profile_spmm_events(start, stop):
 
 __all__ = ["Csr", "spmm", "spmm_factored", "spmm_supports_factored", "spmm_autograd", "gemm", "gemm_supports_a_dropout", "gemm_autograd", "masked_softmax_xent",
            "masked_softmax_xent_autograd", "bernoulli_mask", "dropout_dense",
-           "dropout_dense_autograd", "relu_dropout_bwd", "dropout_philox", "relu_dropout_bwd_philox", "philox_uniform", "gather_rows", "adam_step"]
+           "dropout_dense_autograd", "relu_dropout_bwd", "dropout_philox", "relu_dropout_bwd_philox", "philox_uniform", "gather_rows", "adam_step",
+           "attention", "attention_bwd", "attention_autograd", "norm_residual", "norm_residual_bwd", "norm_residual_autograd",
+           "AdamWState", "adamw_state", "adamw_step"]

@@ -545,6 +545,39 @@ class AdamOptimizer(object):
                               self._step_dev, self.beta1, self.beta2, self.epsilon, weight_decay=wd)
 
 
+class AdamWOptimizer(AdamOptimizer):
+    """Adam with decoupled weight decay over all variables in one launch
+    (:func:`gcn_amd.ops.adamw_step`), its moments in 32 or in 8 bits
+    (``state_bits``; for weights of a graph's size, the first layer of a featureless
+    model).  Weight-decay terms of the loss stay what they are, a gradient."""
+
+    def __init__(self, learning_rate=0.001, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, state_bits=32, seed=0):
+        super(AdamWOptimizer, self).__init__(learning_rate, beta1, beta2, epsilon)
+        self.weight_decay, self.state_bits, self.seed = weight_decay, state_bits, seed
+        self._state = None     # (the variables' tensors, their moments)
+
+    def apply(self, variables, grads, decay=None):
+        decay = decay or {}
+        tensors = [v.tensor for v in variables]
+        if self._state is None or len(self._state[0]) != len(tensors) or any(a is not b for a, b in zip(self._state[0], tensors)):
+            # new storage (a variable initialised or loaded): new moments, as Variable.load says
+            self._state = (tensors, ops.adamw_state(tensors, self.state_bits, self.seed))
+        if self._step_dev is None:
+            self._step_dev = ops.device_counter(device(), self.step)
+        if not torch.cuda.is_current_stream_capturing():
+            self.step += 1
+        ops.counter_add(self._step_dev, 1)
+        full = []
+        with torch.no_grad():
+            for v, g in zip(variables, grads):
+                coef = decay.get(v, 0.0)
+                if coef:
+                    g = v.tensor * coef if g is None else g.add(v.tensor, alpha=coef)
+                full.append(g.contiguous() if g is not None else None)
+            ops.adamw_step(tensors, full, self._state[1], self.learning_rate, self._step_dev, self.beta1, self.beta2, self.epsilon,
+                           self.weight_decay)
+
+
 class _Saver(object):
     def __init__(self, var_dict):
         self.vars = dict(var_dict) if isinstance(var_dict, dict) else {v.name: v for v in var_dict}
@@ -564,6 +597,7 @@ class _Saver(object):
 
 class _Train(object):
     AdamOptimizer = AdamOptimizer
+    AdamWOptimizer = AdamWOptimizer
     Saver = _Saver
 
 

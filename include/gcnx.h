@@ -528,7 +528,8 @@ int gcnx_gemm_dropout_at_rows_f32(int64_t M, int64_t N, int64_t K, const float *
  * elements, other strides in elements (0 allowed, not negative).  Logits, softmax
  * and sums are fp32, results are rounded once.  Sums have a fixed order: results
  * are bitwise reproducible.
- * Rows of more than 512 edges are cut into pieces joined by a second launch.
+ * Long rows (over 256 .. 2048 edges by the size of the matrix) are cut into pieces
+ * joined by a second launch.
  * max_row_nnz, the most edges of a row, says that there are none (0: unknown); it
  * never changes a result beyond that order of sums. */
 typedef enum gcnx_dtype { GCNX_F32 = 0, GCNX_BF16 = 1, GCNX_F16 = 2 } gcnx_dtype;
@@ -568,6 +569,85 @@ int gcnx_attention_backward(const gcnx_attention *p, const int32_t *chunk_row,
                             const float *stats, const void *dout, int64_t dout_row,
                             int64_t dout_head, void *dq, void *dk, void *dv,
                             void *ws, size_t ws_bytes, void *stream);
+
+/* ---- norms around a block, with its gate and residual scale -----------------
+ * No counterpart in the reference (two layers need none).  Rows of dim (1..4096)
+ * elements of x, z, gate (dtype; leading dimensions in elements):
+ *   u = norm(z) * post_weight    y = x + res_scale * sigmoid(gate) * u
+ *   h = norm(y) * pre_weight
+ * norm(a) = (a - mean) / sqrt(mean((a - mean)^2) + eps), mean = 0 unless `layer`.
+ * gate, post_weight (then u = z), res_scale and pre_weight (then no h) may be NULL;
+ * so may z (then y = x: h = norm(x) * pre_weight alone).  Weights are fp32 [dim].
+ * Norms are fp32 over the unrounded values; y and h are rounded once. */
+typedef struct gcnx_norm_residual {
+  int64_t n;
+  int32_t dim;
+  int32_t dtype;              /* gcnx_dtype of x, z, gate, y, h and their gradients */
+  int32_t layer;
+  float eps;
+  const void *x;
+  int64_t x_ld;
+  const void *z;              /* nullable */
+  int64_t z_ld;
+  const void *gate;           /* nullable */
+  int64_t gate_ld;
+  const float *post_weight;   /* nullable */
+  const float *res_scale;     /* nullable */
+  const float *pre_weight;    /* nullable */
+} gcnx_norm_residual;
+/* y is not written without z, h not without pre_weight.  y may be x, or z.
+ * stats (nullable, fp32 [n, 4], 16-byte aligned): what the backward needs. */
+int gcnx_norm_residual_forward(const gcnx_norm_residual *p, void *y, int64_t y_ld,
+                               void *h, int64_t h_ld, float *stats, void *stream);
+/* Gradients for dy (nullable: zero) and dh (nullable: zero).  Any result may be
+ * NULL; dx, dz, dgate are contiguous [n, dim] of dtype, dpost, dres, dpre fp32
+ * [dim], summed over the rows in a fixed order.  The workspace is needed for those
+ * three only. */
+size_t gcnx_norm_residual_backward_workspace_bytes(const gcnx_norm_residual *p);
+int gcnx_norm_residual_backward(const gcnx_norm_residual *p, const void *dy, int64_t dy_ld,
+                                const void *dh, int64_t dh_ld, const float *stats,
+                                void *dx, void *dz, void *dgate, float *dpost,
+                                float *dres, float *dpre, void *ws, size_t ws_bytes,
+                                void *stream);
+
+/* ---- AdamW over many tensors --------------------------------------------------
+ * The many-tensor, decoupled-decay sibling of gcnx_adam_step_f32 (no counterpart in
+ * the reference, which trains two matrices: gcn/models.py:142):
+ *   m = beta1 m + (1 - beta1) g       v = beta2 v + (1 - beta2) g^2
+ *   w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * The tensors of one call share the dtypes of weights and of gradients; every tensor
+ * is contiguous at any alignment of its elements.  The state of all tensors lies in
+ * two arrays: tensor i owns the elements [state, state + n rounded up to
+ * GCNX_ADAMW_BLOCK), state being a multiple of that; elements behind n are zero and
+ * stay so.  state_bits 32: fp32 m and v.  8: e4m3 (OCP) codes of m / scale and of
+ * sqrt(v) / scale with one fp32 power-of-two scale per GCNX_ADAMW_BLOCK elements,
+ * rounded by chance (uniform numbers from Philox4x32-10 keyed by seed, counter
+ * (element / 4, t)), positive values of sqrt(v) never to zero; zeroed codes with any
+ * finite scale are the initial state.  t counts from 1; with t_dev it is read from
+ * device memory when the kernels run (for launches recorded in a HIP graph) and a
+ * workspace of GCNX_ADAMW_WORKSPACE_BYTES is needed.  One launch per 64 tensors. */
+#define GCNX_ADAMW_BLOCK 256
+#define GCNX_ADAMW_WORKSPACE_BYTES 256
+typedef struct gcnx_adamw_tensor {
+  void *w;
+  const void *grad;
+  int64_t n;
+  int64_t state;              /* first element of its state */
+  double weight_decay;
+} gcnx_adamw_tensor;
+typedef struct gcnx_adamw {
+  int32_t w_dtype, g_dtype;   /* gcnx_dtype */
+  int32_t state_bits;         /* 32 or 8 */
+  void *exp_avg, *exp_avg_sq; /* 16-byte aligned */
+  float *exp_avg_scale, *exp_avg_sq_scale; /* 8 bits only */
+  double lr, beta1, beta2, eps;
+  int64_t t;
+  const uint64_t *t_dev;      /* nullable */
+  uint64_t seed;
+} gcnx_adamw;
+int gcnx_adamw_step(const gcnx_adamw *p, int64_t n_tensors,
+                    const gcnx_adamw_tensor *h_tensors /* host array */, void *ws,
+                    size_t ws_bytes, void *stream);
 
 /* ---- glue kernels of one training step ------------------------------------ */
 

@@ -94,7 +94,7 @@ def test_pattern_shapes(env, n_rows, n_cols, nnz):
         Case(env, row, col, (n_rows, n_cols), 4, 2, 16, dtype, seed=nnz).check()
 
 
-@pytest.mark.parametrize("edges", [510, 511, 512, 513, 514, 1023, 1024, 1025, 2300])
+@pytest.mark.parametrize("edges", [255, 256, 257, 258, 510, 511, 512, 513, 514, 1023, 1024, 1025, 2300])
 @pytest.mark.parametrize("before", [0, 1, 511, 512, 700, 1024])
 def test_long_rows(env, edges, before):
     """A row cut at multiples of 512 in the order of the nonzeros, and the column of
@@ -106,6 +106,17 @@ def test_long_rows(env, edges, before):
         shape = (9, 50) if r is row else (50, 9)
         Case(env, r, c, shape, 2, 1, 12, "float32", seed=edges).check()
         Case(env, r, c, shape, 2, 2, 16, "bfloat16", seed=edges).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_many_pieces(env, dtype):
+    """More pieces than the lanes that join them take in one go, one row and several."""
+    rng = np.random.RandomState(71)
+    for n_rows in (1, 3):
+        row = rng.randint(0, n_rows, 60000).astype(np.int32)
+        col = rng.randint(0, 700, 60000).astype(np.int32)
+        Case(env, row, col, (n_rows, 700), 2, 1, 12, dtype, seed=3).check()
+        Case(env, col, row, (700, n_rows), 4, 2, 3, dtype, seed=4).check()
 
 
 def test_row_length_hint_changes_nothing(env):

@@ -165,7 +165,7 @@ SIGNATURES = {
     "gcnx_norm_residual_forward": (_int, [_nrm_p, _p, _i64, _p, _i64, _p, _p]),
     "gcnx_norm_residual_backward_workspace_bytes": (_sz, [_nrm_p]),
     "gcnx_norm_residual_backward": (_int, [_nrm_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
-    "gcnx_adamw_step": (_int, [C.POINTER(AdamWStruct), _i64, C.POINTER(AdamWTensorStruct), _p, _sz, _p]),
+    "gcnx_adamw_step": (_int, [C.POINTER(AdamWStruct), _i64, _p, _p, _sz, _p]),
     "gcnx_xent_workspace_bytes": (_sz, [_i64]),
     "gcnx_masked_softmax_xent_f32": (_int, [_i64, _i32, _p, _i64, _p, _i64, _p, _f64, _p, _p, _i64,
                                             _p, _sz, _p]),

@@ -472,42 +472,47 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 
 
 def _check_heads(t, name, rows, dim=None, like=None):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    """The strides of [rows, heads, head_dim] with contiguous head vectors."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError("%s must be a CUDA (ROCm) tensor; gcn_amd has no CPU path" % name)
-    if t.dtype not in _DTYPES:
-        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1 and t.numel()):
+    dtype, shape, stride = t.dtype, t.shape, t.stride()
+    if dtype not in _DTYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, dtype))
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1 and t.numel()):
         raise ValueError("%s must be [rows, heads, head_dim] with contiguous head vectors" % name)
-    if t.shape[0] != rows:
-        raise ValueError("%s has %d rows, the matrix asks for %d" % (name, t.shape[0], rows))
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if shape[0] != rows:
+        raise ValueError("%s has %d rows, the matrix asks for %d" % (name, shape[0], rows))
+    if like is not None and (dtype != like.dtype or t.device != like.device):
         raise ValueError("%s differs in dtype or device" % name)
-    if dim is not None and t.shape[2] != dim:
-        raise ValueError("%s has head_dim %d, expected %d" % (name, t.shape[2], dim))
+    if dim is not None and shape[2] != dim:
+        raise ValueError("%s has head_dim %d, expected %d" % (name, shape[2], dim))
+    return stride
 
 
 def _attention_struct(a, q, k, v, scale, use_values, mask):
-    _check_heads(q, "q", a.n_rows)
-    _check_heads(k, "k", a.n_cols, q.shape[2], q)
-    _check_heads(v, "v", a.n_cols, q.shape[2], q)
+    qs = _check_heads(q, "q", a.n_rows)
+    _, heads, dim = q.shape
+    ks = _check_heads(k, "k", a.n_cols, dim, q)
+    vs = _check_heads(v, "v", a.n_cols, dim, q)
     if q.device != a.device:
         raise ValueError("the matrix and q live on different devices")
-    heads, kv, dim = q.shape[1], k.shape[1], q.shape[2]
+    kv = k.shape[1]
     if v.shape[1] != kv or kv < 1 or heads < 1 or heads % kv:
         raise ValueError("%d query heads cannot share %d key and %d value heads" % (heads, kv, v.shape[1]))
     if not 1 <= dim <= 256:
         raise ValueError("head_dim must be 1..256, got %d" % dim)
-    midx = None
+    mask_ptr = index_ptr = None
     if mask is not None:
         if mask.dtype != torch.uint8 or mask.dim() != 1 or mask.numel() != a.nnz or not mask.is_contiguous() or \
                 mask.device != a.device:
             raise ValueError("mask must be contiguous uint8 with one byte per nonzero on A's device")
-        midx = a.input_index
+        mask_ptr = mask.data_ptr()
+        if a.input_index is not None:
+            index_ptr = a.input_index.data_ptr()
     return _lib.AttentionStruct(
-        C.pointer(a._struct), int(bool(use_values)), _DTYPES[q.dtype], mask.data_ptr() if mask is not None else None,
-        midx.data_ptr() if midx is not None else None, a.max_row_nnz(), heads, kv, dim,
-        float(scale) if scale is not None else dim ** -0.5, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-        k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1))
+        C.pointer(a._struct), 1 if use_values else 0, _DTYPES[q.dtype], mask_ptr, index_ptr, a.max_row_nnz(), heads, kv, dim,
+        dim ** -0.5 if scale is None else scale, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+        vs[1])
 
 
 _HERE = contextlib.nullcontext()
@@ -516,6 +521,16 @@ _HERE = contextlib.nullcontext()
 def _on(device):
     """Makes ``device`` current for the launches of a ``with`` block."""
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream_of(device):
+    """The current stream of ``device`` as the C ABI takes it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _at(t):
+    """Address of a tensor or None."""
+    return None if t is None else t.data_ptr()
 
 
 def _scratch(nbytes, device):
@@ -538,17 +553,20 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
     (reference gcn/layers.py:219 sums the neighbours with fixed weights)."""
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
+    dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        os = out.stride()
     else:
-        _check_heads(out, "out", a.n_rows, q.shape[2], q)
-        if out.shape[1] != q.shape[1] or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        os = _check_heads(out, "out", a.n_rows, q.shape[2], q)
+        if out.shape[1] != q.shape[1] or any(s == 0 and n > 1 for s, n in zip(os, out.shape)):
             raise ValueError("out must be [n_rows, heads, head_dim] of distinct elements")
-    stats = torch.empty((a.n_rows, q.shape[1], 2), dtype=torch.float32, device=q.device) if want_stats else None
-    with _on(q.device):
-        ws = _scratch(lib.gcnx_attention_workspace_bytes(C.byref(p)), q.device)
-        _lib.check(lib.gcnx_attention_forward(C.byref(p), _ptr(a.chunk_row), _ptr(out), out.stride(0), out.stride(1),
-                                              _ptr(stats), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+    stats = torch.empty((a.n_rows, q.shape[1], 2), dtype=torch.float32, device=dev) if want_stats else None
+    with _on(dev):
+        need = lib.gcnx_attention_workspace_bytes(C.byref(p))
+        ws = _scratch(need, dev)
+        _lib.check(lib.gcnx_attention_forward(C.byref(p), a.chunk_row.data_ptr(), out.data_ptr(), os[0], os[1], _at(stats), _at(ws),
+                                              need, _stream_of(dev)))
     return (out, stats) if want_stats else out
 
 
@@ -560,26 +578,29 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
     Uses the transpose of ``a`` (built at its first use)."""
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
-    for t, name in ((out, "out"), (d_out, "d_out")):
-        _check_heads(t, name, a.n_rows, q.shape[2], q)
-        if t.shape[1] != q.shape[1]:
-            raise ValueError("%s has %d heads, expected %d" % (name, t.shape[1], q.shape[1]))
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (a.n_rows, q.shape[1], 2) or not stats.is_contiguous() or \
-            stats.device != q.device:
+    dev, dim = q.device, q.shape[2]
+    os = _check_heads(out, "out", a.n_rows, dim, q)
+    gs = _check_heads(d_out, "d_out", a.n_rows, dim, q)
+    if out.shape[1] != q.shape[1] or d_out.shape[1] != q.shape[1]:
+        raise ValueError("out and d_out must have the %d heads of q" % q.shape[1])
+    if stats.dtype != torch.float32 or stats.shape != (a.n_rows, q.shape[1], 2) or not stats.is_contiguous() or \
+            stats.device != dev:
         raise ValueError("stats must be what attention(..., want_stats=True) returned")
     if not need_q and not need_kv:
         return None, None, None
     at = a.transpose()
-    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)
-    dq = new(q) if need_q else None
-    dk, dv = (new(k), new(v)) if need_kv else (None, None)
-    midx = at.input_index if mask is not None else None
-    with _on(q.device):
-        ws = _scratch(lib.gcnx_attention_backward_workspace_bytes(C.byref(p), at.max_row_nnz()), q.device)
+    longest = at.max_row_nnz()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
+    dk = dv = None
+    if need_kv:
+        dk, dv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=q.dtype, device=dev)
+    with _on(dev):
+        need = lib.gcnx_attention_backward_workspace_bytes(C.byref(p), longest)
+        ws = _scratch(need, dev)
         _lib.check(lib.gcnx_attention_backward(
-            C.byref(p), _ptr(a.chunk_row), at.struct_ref(), _ptr(at.chunk_row), _ptr(midx), at.max_row_nnz(), _ptr(out),
-            out.stride(0), out.stride(1), _ptr(stats), _ptr(d_out), d_out.stride(0), d_out.stride(1), _ptr(dq), _ptr(dk),
-            _ptr(dv), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+            C.byref(p), a.chunk_row.data_ptr(), at.struct_ref(), at.chunk_row.data_ptr(),
+            _at(at.input_index) if mask is not None else None, longest, out.data_ptr(), os[0], os[1], stats.data_ptr(),
+            d_out.data_ptr(), gs[0], gs[1], _at(dq), _at(dk), _at(dv), _at(ws), need, _stream_of(dev)))
     return dq, dk, dv
 
 
@@ -612,43 +633,46 @@ def attention_autograd(a, q, k, v, scale=None, use_values=False, mask=None):
 
 # ----------------------------------------------------------------------- norms
 def _check_rows(t, name, like=None):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    """The leading dimension of row-major [n, dim]."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError("%s must be a CUDA (ROCm) tensor; gcn_amd has no CPU path" % name)
     if t.dtype not in _DTYPES:
         raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1 and t.numel()):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1 and t.numel()):
         raise ValueError("%s must be a row-major 2-D tensor" % name)
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (shape != like.shape or t.dtype != like.dtype or t.device != like.device):
         raise ValueError("%s differs from x in shape, dtype or device" % name)
+    return stride[0]
 
 
 def _check_weight(w, name, x):
+    if w is None:
+        return None
     if w.dtype != torch.float32 or w.dim() != 1 or w.numel() != x.shape[1] or not w.is_contiguous() or w.device != x.device:
         raise ValueError("%s must be contiguous float32 [%d] on x's device" % (name, x.shape[1]))
+    return w.data_ptr()
 
 
 def _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps):
-    _check_rows(x, "x")
+    x_ld = _check_rows(x, "x")
+    n, dim = x.shape
     if kind not in ("rms", "layer"):
         raise ValueError("kind must be 'rms' or 'layer', got %r" % (kind,))
-    if not 1 <= x.shape[1] <= 4096:
-        raise ValueError("rows of 1..4096 elements, got %d" % x.shape[1])
+    if not 1 <= dim <= 4096:
+        raise ValueError("rows of 1..4096 elements, got %d" % dim)
+    z_ld = gate_ld = 0
     if z is not None:
-        _check_rows(z, "z", x)
+        z_ld = _check_rows(z, "z", x)
     elif gate is not None or post_weight is not None or res_scale is not None:
         raise ValueError("gate, post_weight and res_scale belong to z")
     elif pre_weight is None:
         raise ValueError("neither z nor pre_weight: nothing to do")
     if gate is not None:
-        _check_rows(gate, "gate", x)
-    for w, name in ((post_weight, "post_weight"), (res_scale, "res_scale"), (pre_weight, "pre_weight")):
-        if w is not None:
-            _check_weight(w, name, x)
-    ptr = lambda t: t.data_ptr() if t is not None else None
-    ld = lambda t: t.stride(0) if t is not None else 0
-    return _lib.NormResidualStruct(x.shape[0], x.shape[1], _DTYPES[x.dtype], int(kind == "layer"), float(eps), x.data_ptr(),
-                                   x.stride(0), ptr(z), ld(z), ptr(gate), ld(gate), ptr(post_weight), ptr(res_scale),
-                                   ptr(pre_weight))
+        gate_ld = _check_rows(gate, "gate", x)
+    return _lib.NormResidualStruct(n, dim, _DTYPES[x.dtype], 1 if kind == "layer" else 0, eps, x.data_ptr(), x_ld, _at(z), z_ld,
+                                   _at(gate), gate_ld, _check_weight(post_weight, "post_weight", x),
+                                   _check_weight(res_scale, "res_scale", x), _check_weight(pre_weight, "pre_weight", x))
 
 
 def norm_residual(x, z=None, gate=None, post_weight=None, res_scale=None, pre_weight=None, kind="rms", eps=1e-6,
@@ -666,13 +690,14 @@ def norm_residual(x, z=None, gate=None, post_weight=None, res_scale=None, pre_we
     ``want_stats``) is what :func:`norm_residual_bwd` needs."""
     lib = _lib.load()
     p = _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps)
-    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = new() if z is not None else x
-    h = new() if pre_weight is not None else None
-    stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device) if want_stats else None
-    if x.shape[0]:
-        with _on(x.device):
-            _lib.check(lib.gcnx_norm_residual_forward(C.byref(p), _ptr(y), y.stride(0), _ptr(h), x.shape[1], _ptr(stats), _stream()))
+    dev, dtype, shape = x.device, x.dtype, x.shape
+    y = torch.empty(shape, dtype=dtype, device=dev) if z is not None else x
+    h = torch.empty(shape, dtype=dtype, device=dev) if pre_weight is not None else None
+    stats = torch.empty((shape[0], 4), dtype=torch.float32, device=dev) if want_stats else None
+    if shape[0]:
+        with _on(dev):
+            _lib.check(lib.gcnx_norm_residual_forward(C.byref(p), y.data_ptr(), y.stride(0), _at(h), shape[1], _at(stats),
+                                                      _stream_of(dev)))
     return y, h, stats
 
 
@@ -684,30 +709,33 @@ def norm_residual_bwd(x, dy, dh, stats, z=None, gate=None, post_weight=None, res
     over the rows in a fixed order."""
     lib = _lib.load()
     p = _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps)
-    for t, name in ((dy, "dy"), (dh, "dh")):
-        if t is not None:
-            _check_rows(t, name, x)
+    dy_ld = _check_rows(dy, "dy", x) if dy is not None else 0
+    dh_ld = _check_rows(dh, "dh", x) if dh is not None else 0
     if dh is not None and pre_weight is None:
         raise ValueError("dh without pre_weight")
     n, dim = x.shape
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (n, 4) or not stats.is_contiguous() or stats.device != x.device:
+    dev, dtype = x.device, x.dtype
+    if stats.dtype != torch.float32 or stats.shape != (n, 4) or not stats.is_contiguous() or stats.device != dev:
         raise ValueError("stats must be what norm_residual(..., want_stats=True) returned")
-    new = lambda on: torch.empty((n, dim), dtype=x.dtype, device=x.device) if on else None
-    dx, dz, dgate = new(True), new(z is not None), new(gate is not None)
-    sums = [w is not None for w in (post_weight, res_scale, pre_weight)]
-    rows = n > 0 and (sums[0] or sums[1] or dh is not None)
-    # no rows, or no gradient behind pre_weight: a sum over nothing
-    made = [(torch.empty if rows and (i < 2 or dh is not None) else torch.zeros)(dim, dtype=torch.float32, device=x.device)
-            if on else None for i, on in enumerate(sums)]
-    dpost, dres, dpre = made
+    dx = torch.empty((n, dim), dtype=dtype, device=dev)
+    dz = torch.empty((n, dim), dtype=dtype, device=dev) if z is not None else None
+    dgate = torch.empty((n, dim), dtype=dtype, device=dev) if gate is not None else None
+    made = [None, None, None]
+    wanted = [i for i, w in enumerate((post_weight, res_scale, pre_weight)) if w is not None]
+    summed = [i for i in wanted if n and (i < 2 or dh is not None)]
+    if wanted:
+        # one buffer for the (small) gradients of the weights; sums over nothing are zero
+        buf = (torch.empty if len(summed) == len(wanted) else torch.zeros)((len(wanted), dim), dtype=torch.float32, device=dev)
+        for row, i in zip(buf.unbind(0), wanted):
+            made[i] = row
     if n:
-        with _on(x.device):
-            ws = _scratch(lib.gcnx_norm_residual_backward_workspace_bytes(C.byref(p)) if rows else 0, x.device)
+        with _on(dev):
+            need = lib.gcnx_norm_residual_backward_workspace_bytes(C.byref(p)) if summed else 0
+            ws = _scratch(need, dev)
             _lib.check(lib.gcnx_norm_residual_backward(
-                C.byref(p), _ptr(dy), dy.stride(0) if dy is not None else 0, _ptr(dh), dh.stride(0) if dh is not None else 0,
-                _ptr(stats), _ptr(dx), _ptr(dz), _ptr(dgate), _ptr(dpost), _ptr(dres), _ptr(dpre if dh is not None else None),
-                _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
-    return dx, dz, dgate, dpost, dres, dpre
+                C.byref(p), _at(dy), dy_ld, _at(dh), dh_ld, stats.data_ptr(), dx.data_ptr(), _at(dz), _at(dgate), _at(made[0]),
+                _at(made[1]), _at(made[2]) if dh is not None else None, _at(ws), need, _stream_of(dev)))
+    return (dx, dz, dgate) + tuple(made)
 
 
 class _NormResidualFn(torch.autograd.Function):
@@ -1096,14 +1124,12 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
         t_ptr, t_host = None, int(t)
     table = state._table.copy()
     table["w"], table["grad"], table["n"], table["decay"] = w_ptr, g_ptr, sizes, weight_decay
-    ptr = lambda x: x.data_ptr() if x is not None else None
-    p = _lib.AdamWStruct(_DTYPES[dtype], _DTYPES[g_dtype], state.bits, ptr(state.exp_avg), ptr(state.exp_avg_sq),
-                         ptr(state.exp_avg_scale), ptr(state.exp_avg_sq_scale), float(lr), float(beta1), float(beta2), float(eps),
-                         t_host, t_ptr, state.seed)
+    p = _lib.AdamWStruct(_DTYPES[dtype], _DTYPES[g_dtype], state.bits, state.exp_avg.data_ptr(), state.exp_avg_sq.data_ptr(),
+                         _at(state.exp_avg_scale), _at(state.exp_avg_sq_scale), lr, beta1, beta2, eps, t_host, t_ptr, state.seed)
     with _on(dev):
-        ws = _scratch(_lib.ADAMW_WORKSPACE_BYTES if t_ptr else 0, dev)
-        _lib.check(lib.gcnx_adamw_step(C.byref(p), count, table.ctypes.data_as(C.POINTER(_lib.AdamWTensorStruct)), _ptr(ws),
-                                       ws.numel() if ws is not None else 0, _stream()))
+        need = _lib.ADAMW_WORKSPACE_BYTES if t_ptr else 0
+        ws = _scratch(need, dev)
+        _lib.check(lib.gcnx_adamw_step(C.byref(p), count, table.ctypes.data, _at(ws), need, _stream_of(dev)))
     return params
 
 

@@ -43,7 +43,11 @@ __device__ __forceinline__ float dot_piece(const typename Piece<T>::raw &a, cons
 
 __device__ __forceinline__ bool is_lowest(float x) { return x == -__builtin_inff(); }
 
-constexpr int kUnroll = 4;   // edges in flight per lane
+// Edges in flight per lane: more cost registers, so wavefronts, and idle slots at the
+// ends of rows.  1 / 2 / 4, us at 2^19 nodes: forward 1082 / 1057 / 1075, row pass
+// 1176 / 1257 / 1406, column pass 1317 / 1394 / 1645.
+constexpr int kForwardEdges = 2;
+constexpr int kBackwardEdges = 1;
 
 struct AttnArgs {
   // pattern walked by this pass (the matrix, or its transpose)
@@ -236,26 +240,26 @@ __global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
   float acc[N] = {}, m = -__builtin_inff(), l = 0.0f;
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (t.count) {
-    Edge<SHIFTS> next[kUnroll];
+    Edge<SHIFTS> next[kForwardEdges];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, t.edge + u * t.edges);
-    for (uint32_t x = t.edge; x < t.count; x += kUnroll * t.edges) {
-      raw k[kUnroll], v[kUnroll];
-      float s[kUnroll];
-      bool on[kUnroll];
+    for (int u = 0; u < kForwardEdges; ++u) next[u].read(p, t, t.edge + u * t.edges);
+    for (uint32_t x = t.edge; x < t.count; x += kForwardEdges * t.edges) {
+      raw k[kForwardEdges], v[kForwardEdges];
+      float s[kForwardEdges];
+      bool on[kForwardEdges];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kForwardEdges; ++u) {
         on[u] = next[u].on;
         s[u] = next[u].shift;
         k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, next[u].col, p.k_bytes), on[u] && t.live), p.dim);
         v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, next[u].col, p.v_bytes), on[u] && t.live), p.dim);
       }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, x + (kUnroll + u) * t.edges);
+      for (int u = 0; u < kForwardEdges; ++u) next[u].read(p, t, x + (kForwardEdges + u) * t.edges);
       read_ahead_fence();
       float top = m;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kForwardEdges; ++u) {
         const float d = group_sum<LPH>(dot_piece<T>(q, k[u]));
         s[u] = on[u] ? fmaf(d, p.scale, s[u]) : -__builtin_inff();
         top = fmaxf(top, s[u]);
@@ -267,7 +271,7 @@ __global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] *= keep;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kForwardEdges; ++u) {
         const float w = exp_of(s[u] - safe);
         l += w;
 #pragma unroll
@@ -427,25 +431,25 @@ __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArg
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (!kCorrected<T> && !p.o0) t.count = 0;        // delta alone is asked for
   if (t.count) {
-    Edge<SHIFTS> next[kUnroll];
+    Edge<SHIFTS> next[kBackwardEdges];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, t.edge + u * t.edges);
-    for (uint32_t x = t.edge; x < t.count; x += kUnroll * t.edges) {
-      raw k[kUnroll], v[kUnroll];
-      float shift[kUnroll];
-      bool on[kUnroll];
+    for (int u = 0; u < kBackwardEdges; ++u) next[u].read(p, t, t.edge + u * t.edges);
+    for (uint32_t x = t.edge; x < t.count; x += kBackwardEdges * t.edges) {
+      raw k[kBackwardEdges], v[kBackwardEdges];
+      float shift[kBackwardEdges];
+      bool on[kBackwardEdges];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kBackwardEdges; ++u) {
         on[u] = next[u].on;
         shift[u] = next[u].shift;
         k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, next[u].col, p.k_bytes), on[u] && t.live), p.dim);
         v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, next[u].col, p.v_bytes), on[u] && t.live), p.dim);
       }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) next[u].read(p, t, x + (kUnroll + u) * t.edges);
+      for (int u = 0; u < kBackwardEdges; ++u) next[u].read(p, t, x + (kBackwardEdges + u) * t.edges);
       read_ahead_fence();
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kBackwardEdges; ++u) {
         const float s = group_sum<LPH>(dot_piece<T>(q, k[u])), d = group_sum<LPH>(dot_piece<T>(g, v[u]));
         const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r : 0.0f;
         const float ds = on[u] ? w * (d - d0) : 0.0f;
@@ -499,8 +503,8 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
     // item x is edge x / group under query head x % group
     uint32_t at = t.edge / group, sub = t.edge - at * group;
     const uint32_t at_step = t.edges / group, sub_step = t.edges - at_step * group;
-    Edge<SHIFTS> next[kUnroll];
-    uint32_t next_sub[kUnroll];
+    Edge<SHIFTS> next[kBackwardEdges];
+    uint32_t next_sub[kBackwardEdges];
     auto read = [&](int u) {
       next[u].read(p, t, at);
       next_sub[u] = sub;
@@ -512,14 +516,14 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
       }
     };
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) read(u);
+    for (int u = 0; u < kBackwardEdges; ++u) read(u);
     for (uint32_t first = t.edge / group; first < t.count;) {
-      raw q[kUnroll], g[kUnroll];
-      f32x4 st[kUnroll];
-      float shift[kUnroll];
-      bool on[kUnroll];
+      raw q[kBackwardEdges], g[kBackwardEdges];
+      f32x4 st[kBackwardEdges];
+      float shift[kBackwardEdges];
+      bool on[kBackwardEdges];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kBackwardEdges; ++u) {
         on[u] = next[u].on;
         shift[u] = next[u].shift;
         const bool there = on[u] && t.live;
@@ -530,10 +534,10 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
       }
       first = at;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) read(u);
+      for (int u = 0; u < kBackwardEdges; ++u) read(u);
       read_ahead_fence();
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kBackwardEdges; ++u) {
         const float s = group_sum<LPH>(dot_piece<T>(k, q[u])), d = group_sum<LPH>(dot_piece<T>(v, g[u]));
         const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - st[u][0]) * st[u][1] : 0.0f;
         const float ds = on[u] ? w * (d - st[u][2]) : 0.0f;
@@ -712,11 +716,12 @@ static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   const int spare = slots_log2 - p.heads_log2;
   // edges side by side, what is left takes further rows: as many edges as the average
   // row has, so that rows end soon, unless there are rows enough to fill the machine
-  // (8 wavefronts a SIMD): then kUnroll edges a lane, so that few lanes idle.
-  // (Cora: 11 us against 18 with kUnroll; 2^18 rows of 2: 285 against 160.)
+  // (8 wavefronts a SIMD): then as many rounds as a lane has edges in
+  // flight, so that few lanes idle.  (Cora, 4 edges in flight: 11 us against 18; 2^18
+  // rows of 2: 285 against 160.)
   const int64_t items = ceil_div(p.nnz * (pass == kBackwardColumns ? p.group : 1), p.n_rows);
   int e = log2_ceil(items);
-  if ((p.n_rows << (e < spare ? e : spare)) >> spare > 8 * 1024) e = log2_ceil(ceil_div(items, kUnroll));
+  if ((p.n_rows << (e < spare ? e : spare)) >> spare > 8 * 1024) e = log2_ceil(ceil_div(items, pass == kForward ? kForwardEdges : kBackwardEdges));
   p.edge_log2 = e < spare ? e : spare;
   p.row_log2 = spare - p.edge_log2;
   p.tiles = (int)ceil_div(heads, (int64_t)1 << p.heads_log2);

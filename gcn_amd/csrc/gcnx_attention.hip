@@ -49,6 +49,12 @@ __device__ __forceinline__ bool is_lowest(float x) { return x == -__builtin_inff
 constexpr int kForwardEdges = 2;
 constexpr int kBackwardEdges = 1;
 
+// Wavefronts a SIMD that the registers have to leave room for: 8 (64 registers) where
+// nothing is spilled for it.  (Column pass at 2^19 nodes: 1284 us against 1525 with
+// the 5 that the compiler chooses.)
+template <int LPH, bool SHIFTS>
+constexpr int kWaves = SHIFTS || LPH == 0 || LPH >= 32 ? 6 : 8;
+
 struct AttnArgs {
   // pattern walked by this pass (the matrix, or its transpose)
   const int64_t *row_ptr;
@@ -164,26 +170,70 @@ __device__ __forceinline__ bool find_task(const AttnArgs &p, int heads, Task &t)
   return true;
 }
 
-// The edges of the next turn, read one turn ahead: their columns, logit shifts, and
-// whether they take part.  An edge whose shift is -inf is out of the softmax like a
-// masked one: its operands are not read, so infinities and NaN in masked places
-// stay where they are.  SHIFTS: there are values or a mask.
+// An edge, read a turn before it is used: its column, its logit shift, whether it
+// takes part.  An edge whose shift is -inf is out of the softmax like a masked one:
+// its operands are not read, so infinities and NaN in masked places stay where they
+// are.  SHIFTS: there are values or a mask; the mask's index is then read two turns
+// ahead, its byte one.  What is read is not looked at before its turn, so that
+// nothing waits for it.
 template <bool SHIFTS>
 struct Edge {
   int32_t col;
   float shift;
-  bool on;
-  __device__ __forceinline__ void read(const AttnArgs &p, const Task &t, uint32_t x) {
-    on = x < t.count;
-    const int64_t e = t.beg + (on ? x : 0);       // t.count > 0: edge 0 is there
+  uint32_t keep;
+  bool there;
+  int64_t index;
+  __device__ __forceinline__ void start(const AttnArgs &p, const Task &t, uint32_t x) {
+    there = x < t.count;
+    const int64_t e = t.beg + (there ? x : 0);       // t.count > 0: edge 0 is there
     col = p.col_idx[e];
     shift = 0.0f;
+    keep = 1;
     if constexpr (SHIFTS) {
-      if (p.val) {
-        shift = p.val[e];
-        on = on && !is_lowest(shift);
+      if (p.val) shift = p.val[e];
+      index = e;
+      if (p.mask_index) index = p.mask_index[e];
+    }
+  }
+  __device__ __forceinline__ void check(const AttnArgs &p) {
+    if constexpr (SHIFTS)
+      if (p.mask) keep = p.mask[index];
+  }
+  __device__ __forceinline__ bool on() const { return there && (!SHIFTS || (keep != 0 && !is_lowest(shift))); }
+};
+
+// U edges a turn; place(u) is the place in the row of the u-th edge to read.
+template <bool SHIFTS, int U>
+struct Edges {
+  Edge<SHIFTS> next[U], later[U];
+  __device__ __forceinline__ bool more() const { return next[0].there; }
+  template <typename Place>
+  __device__ __forceinline__ void begin(const AttnArgs &p, const Task &t, Place place) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u].start(p, t, place(u));
+    if constexpr (SHIFTS) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) later[u].start(p, t, place(U + u));
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u].check(p);
+    }
+  }
+  // place(u): of the edge that comes `ahead` turns after this one
+  static constexpr int ahead = SHIFTS ? 2 : 1;
+  template <typename Place>
+  __device__ __forceinline__ void advance(const AttnArgs &p, const Task &t, Place place) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (SHIFTS) {
+        next[u] = later[u];
+        later[u].start(p, t, place(u));
+      } else {
+        next[u].start(p, t, place(u));
       }
-      if (p.mask) on = on && p.mask[p.mask_index ? p.mask_index[e] : e] != 0;
+    }
+    if constexpr (SHIFTS) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u].check(p);
     }
   }
 };
@@ -230,7 +280,7 @@ template <typename T, int LPH>
 constexpr int kPartWide = (LPH ? LPH : 1) * Piece<T>::N;
 
 template <typename T, int LPH, bool SHIFTS>
-__global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forward_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   Task t;
@@ -240,22 +290,20 @@ __global__ __launch_bounds__(kBlock) void attention_forward_kernel(AttnArgs p) {
   float acc[N] = {}, m = -__builtin_inff(), l = 0.0f;
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (t.count) {
-    Edge<SHIFTS> next[kForwardEdges];
-#pragma unroll
-    for (int u = 0; u < kForwardEdges; ++u) next[u].read(p, t, t.edge + u * t.edges);
-    for (uint32_t x = t.edge; x < t.count; x += kForwardEdges * t.edges) {
+    Edges<SHIFTS, kForwardEdges> edges;
+    edges.begin(p, t, [&](int u) { return t.edge + u * t.edges; });
+    for (uint32_t x = t.edge; edges.more(); x += kForwardEdges * t.edges) {
       raw k[kForwardEdges], v[kForwardEdges];
       float s[kForwardEdges];
       bool on[kForwardEdges];
 #pragma unroll
       for (int u = 0; u < kForwardEdges; ++u) {
-        on[u] = next[u].on;
-        s[u] = next[u].shift;
-        k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, next[u].col, p.k_bytes), on[u] && t.live), p.dim);
-        v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, next[u].col, p.v_bytes), on[u] && t.live), p.dim);
+        on[u] = edges.next[u].on();
+        s[u] = edges.next[u].shift;
+        k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, edges.next[u].col, p.k_bytes), on[u] && t.live), p.dim);
+        v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, edges.next[u].col, p.v_bytes), on[u] && t.live), p.dim);
       }
-#pragma unroll
-      for (int u = 0; u < kForwardEdges; ++u) next[u].read(p, t, x + (kForwardEdges + u) * t.edges);
+      edges.advance(p, t, [&](int u) { return x + (edges.ahead * kForwardEdges + u) * t.edges; });
       read_ahead_fence();
       float top = m;
 #pragma unroll
@@ -420,7 +468,7 @@ __device__ __forceinline__ typename Piece<T>::raw load_row(const AttnArgs &p, co
 }
 
 template <typename T, int LPH, bool SHIFTS>
-__global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArgs p) {
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_rows_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   Task t;
@@ -431,22 +479,20 @@ __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArg
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (!kCorrected<T> && !p.o0) t.count = 0;        // delta alone is asked for
   if (t.count) {
-    Edge<SHIFTS> next[kBackwardEdges];
-#pragma unroll
-    for (int u = 0; u < kBackwardEdges; ++u) next[u].read(p, t, t.edge + u * t.edges);
-    for (uint32_t x = t.edge; x < t.count; x += kBackwardEdges * t.edges) {
+    Edges<SHIFTS, kBackwardEdges> edges;
+    edges.begin(p, t, [&](int u) { return t.edge + u * t.edges; });
+    for (uint32_t x = t.edge; edges.more(); x += kBackwardEdges * t.edges) {
       raw k[kBackwardEdges], v[kBackwardEdges];
       float shift[kBackwardEdges];
       bool on[kBackwardEdges];
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
-        on[u] = next[u].on;
-        shift[u] = next[u].shift;
-        k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, next[u].col, p.k_bytes), on[u] && t.live), p.dim);
-        v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, next[u].col, p.v_bytes), on[u] && t.live), p.dim);
+        on[u] = edges.next[u].on();
+        shift[u] = edges.next[u].shift;
+        k[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(kb, edges.next[u].col, p.k_bytes), on[u] && t.live), p.dim);
+        v[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(vb, edges.next[u].col, p.v_bytes), on[u] && t.live), p.dim);
       }
-#pragma unroll
-      for (int u = 0; u < kBackwardEdges; ++u) next[u].read(p, t, x + (kBackwardEdges + u) * t.edges);
+      edges.advance(p, t, [&](int u) { return x + (edges.ahead * kBackwardEdges + u) * t.edges; });
       read_ahead_fence();
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
@@ -488,7 +534,7 @@ __global__ __launch_bounds__(kBlock) void attention_backward_rows_kernel(AttnArg
 // the key heads; the edges of the column are walked once per query head that
 // shares the key head, as count * group items.
 template <typename T, int LPH, bool SHIFTS>
-__global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(AttnArgs p) {
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_columns_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   Task t;
@@ -500,41 +546,44 @@ __global__ __launch_bounds__(kBlock) void attention_backward_columns_kernel(Attn
                 stb = (Address)(p.stats4 + head0);
   if (t.count) {
     const uint32_t group = p.group;
-    // item x is edge x / group under query head x % group
+    // item x is edge x / group under query head x % group; `at`, `sub`: the next to read
     uint32_t at = t.edge / group, sub = t.edge - at * group;
     const uint32_t at_step = t.edges / group, sub_step = t.edges - at_step * group;
-    Edge<SHIFTS> next[kBackwardEdges];
-    uint32_t next_sub[kBackwardEdges];
-    auto read = [&](int u) {
-      next[u].read(p, t, at);
-      next_sub[u] = sub;
+    constexpr int U = kBackwardEdges;
+    Edges<SHIFTS, U> edges;
+    uint32_t subs[2 * U];                          // query heads of the next edges and of the later ones
+    const auto place = [&](int to) {
+      const uint32_t x = at;
+      subs[to] = sub;
       at += at_step;
       sub += sub_step;
       if (sub >= group) {
         sub -= group;
         ++at;
       }
+      return x;
     };
-#pragma unroll
-    for (int u = 0; u < kBackwardEdges; ++u) read(u);
-    for (uint32_t first = t.edge / group; first < t.count;) {
+    edges.begin(p, t, place);
+    while (edges.more()) {
       raw q[kBackwardEdges], g[kBackwardEdges];
       f32x4 st[kBackwardEdges];
       float shift[kBackwardEdges];
       bool on[kBackwardEdges];
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
-        on[u] = next[u].on;
-        shift[u] = next[u].shift;
+        on[u] = edges.next[u].on();
+        shift[u] = edges.next[u].shift;
         const bool there = on[u] && t.live;
-        const int32_t row = next[u].col, h = next_sub[u];
+        const int32_t row = edges.next[u].col, h = subs[u];
         q[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(row_at(qb, row, p.q_bytes), h, p.q_head_bytes), there), p.dim);
         g[u] = load_piece<T, LPH == 0>(at_or_zeros(row_at(row_at(gb, row, p.dout_bytes), h, p.dout_head_bytes), there), p.dim);
         st[u] = load_at<f32x4>(at_or_zeros(row_at(stb, row, p.heads * 16) + h * 16, there));
       }
-      first = at;
+      if (SHIFTS) {
 #pragma unroll
-      for (int u = 0; u < kBackwardEdges; ++u) read(u);
+        for (int u = 0; u < U; ++u) subs[u] = subs[U + u];
+      }
+      edges.advance(p, t, [&](int u) { return place((edges.ahead - 1) * U + u); });
       read_ahead_fence();
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {

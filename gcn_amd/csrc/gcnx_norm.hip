@@ -354,7 +354,7 @@ static int64_t norm_blocks(int64_t n, int tpr, int64_t deep) {
   const int64_t every = ceil_div(n, rows_per_block(tpr)), most = 256 * deep * kBlock / (tpr > kWave ? tpr : kBlock);
   return every < most ? every : most;
 }
-constexpr int64_t kForwardDeep = 8, kBackwardDeep = 4;
+constexpr int64_t kForwardDeep = 3, kBackwardDeep = 2;
 
 template <typename T, bool LAYER>
 static void launch_norm(bool backward, int tpr, int64_t blocks, const NormArgs &p, hipStream_t stream) {

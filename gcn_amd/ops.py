@@ -533,6 +533,11 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _like(t):
+    """An uninitialised contiguous tensor of t's shape and type (the cheapest call for it)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _scratch(nbytes, device):
     # from torch's allocator, which orders the memory by stream and owns it in a
     # capture: two streams, or two recorded graphs, never share it
@@ -555,7 +560,7 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
     dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = _like(q)
         os = out.stride()
     else:
         os = _check_heads(out, "out", a.n_rows, q.shape[2], q)
@@ -590,10 +595,10 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
         return None, None, None
     at = a.transpose()
     longest = at.max_row_nnz()
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
+    dq = _like(q) if need_q else None
     dk = dv = None
     if need_kv:
-        dk, dv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(k.shape, dtype=q.dtype, device=dev)
+        dk, dv = _like(k), _like(v)
     with _on(dev):
         need = lib.gcnx_attention_backward_workspace_bytes(C.byref(p), longest)
         ws = _scratch(need, dev)
@@ -690,9 +695,9 @@ def norm_residual(x, z=None, gate=None, post_weight=None, res_scale=None, pre_we
     ``want_stats``) is what :func:`norm_residual_bwd` needs."""
     lib = _lib.load()
     p = _norm_struct(x, z, gate, post_weight, res_scale, pre_weight, kind, eps)
-    dev, dtype, shape = x.device, x.dtype, x.shape
-    y = torch.empty(shape, dtype=dtype, device=dev) if z is not None else x
-    h = torch.empty(shape, dtype=dtype, device=dev) if pre_weight is not None else None
+    dev, shape = x.device, x.shape
+    y = _like(x) if z is not None else x
+    h = _like(x) if pre_weight is not None else None
     stats = torch.empty((shape[0], 4), dtype=torch.float32, device=dev) if want_stats else None
     if shape[0]:
         with _on(dev):
@@ -714,12 +719,12 @@ def norm_residual_bwd(x, dy, dh, stats, z=None, gate=None, post_weight=None, res
     if dh is not None and pre_weight is None:
         raise ValueError("dh without pre_weight")
     n, dim = x.shape
-    dev, dtype = x.device, x.dtype
+    dev = x.device
     if stats.dtype != torch.float32 or stats.shape != (n, 4) or not stats.is_contiguous() or stats.device != dev:
         raise ValueError("stats must be what norm_residual(..., want_stats=True) returned")
-    dx = torch.empty((n, dim), dtype=dtype, device=dev)
-    dz = torch.empty((n, dim), dtype=dtype, device=dev) if z is not None else None
-    dgate = torch.empty((n, dim), dtype=dtype, device=dev) if gate is not None else None
+    dx = _like(x)
+    dz = _like(x) if z is not None else None
+    dgate = _like(x) if gate is not None else None
     made = [None, None, None]
     wanted = [i for i, w in enumerate((post_weight, res_scale, pre_weight)) if w is not None]
     summed = [i for i in wanted if n and (i < 2 or dh is not None)]

@@ -77,8 +77,9 @@ struct AttnArgs {
   f32x4 *stats4;                // backward: m, r, delta per row and head
   // work split
   float *part;                  // partial results of cut rows
-  int64_t part_floats;          // per piece
-  int64_t n_pieces;             // 2 * chunks of `segment` nonzeros, 0: no row is cut
+  int64_t part_floats;          // per piece; 0: no pieces
+  int64_t n_pieces;             // tasks of cut rows, before those of the others
+  bool whole;                   // a cut row is one workgroup's (4 tasks a chunk), else pieces (2 tasks a chunk)
   int32_t segment;              // rows longer than this are cut at its multiples
   int32_t heads_log2;           // heads side by side in a wavefront (a tile)
   int32_t edge_log2, row_log2;  // edges of a row, rows side by side in a wavefront
@@ -90,8 +91,11 @@ struct Task {
   int64_t row, beg;
   uint32_t count;               // edges from beg on
   int64_t piece;                // >= 0: a piece of a cut row
+  bool whole;                   // the workgroup's wavefronts share the row
   bool live;                    // the lane has a head and a row to write
-  int32_t edge, edges;          // this lane's place among the edges side by side
+  int32_t edge, edges;          // this lane's first edge, and the edges read side by side
+  int32_t side;                 // of them in this wavefront
+  bool first;                   // the lane that holds the wavefront's sums
   int32_t head, d0, skip;       // head, first element of the lane's piece, elements counted by another lane
 };
 
@@ -129,21 +133,27 @@ template <typename T, int LPH>
 __device__ __forceinline__ bool find_task(const AttnArgs &p, int heads, Task &t) {
   constexpr int L = LPH ? LPH : 1;
   int tile, slot;
-  const int64_t task = tile_of(p, tile) * kWavesPerBlock + (threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);     // tasks are in scalar registers
+  const int64_t task = tile_of(p, tile) * kWavesPerBlock + wave;
   place_lane<T, LPH>(p, heads, tile, t, slot);
   int64_t end;
+  t.piece = -1;
+  t.whole = false;
+  t.first = slot == 0;
   if (task < p.n_pieces) {
-    t.edge = slot;
-    t.edges = (kWave / L) >> p.heads_log2;
-    const int64_t first = (task >> 1) * p.segment, next = first + p.segment;
-    if (task & 1) {             // the cut row that begins in this chunk
+    t.side = (kWave / L) >> p.heads_log2;
+    t.whole = p.whole;
+    t.edge = p.whole ? slot + wave * t.side : slot;
+    t.edges = p.whole ? t.side * kWavesPerBlock : t.side;
+    const int64_t first = (p.whole ? task >> 2 : task >> 1) * p.segment, next = first + p.segment;
+    if (p.whole || (task & 1)) {        // the cut row that begins in this chunk
       if (next >= p.nnz) return false;
       t.row = p.chunk_row[next / kChunkUnit];
       t.beg = p.row_ptr[t.row];
       end = p.row_ptr[t.row + 1];
       if (t.beg < first || t.beg >= next || end - t.beg <= p.segment) return false;
-      end = next;
-    } else {                    // the cut row that goes on into this chunk
+      if (!p.whole) end = next;
+    } else {                            // the cut row that goes on into this chunk
       t.row = p.chunk_row[first / kChunkUnit];
       t.beg = p.row_ptr[t.row];
       end = p.row_ptr[t.row + 1];
@@ -151,12 +161,12 @@ __device__ __forceinline__ bool find_task(const AttnArgs &p, int heads, Task &t)
       t.beg = first;
       end = end < next ? end : next;
     }
-    t.piece = task;
+    if (!p.whole) t.piece = task;
   } else {
     t.edge = slot & ((1 << p.edge_log2) - 1);
-    t.edges = 1 << p.edge_log2;
+    t.side = t.edges = 1 << p.edge_log2;
+    t.first = t.edge == 0;
     t.row = ((task - p.n_pieces) << p.row_log2) + (slot >> p.edge_log2);
-    t.piece = -1;
     const bool there = t.row < p.n_rows;
     if (!there) t.row = p.n_rows - 1;
     t.beg = p.row_ptr[t.row];
@@ -283,6 +293,7 @@ template <typename T, int LPH, bool SHIFTS>
 __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forward_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
+  __shared__ float sh[N + 2][kWave];
   Task t;
   if (!find_task<T, LPH>(p, p.heads, t)) return;
   const int kv = t.head / p.group;
@@ -327,14 +338,37 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forwa
       }
     }
   }
-  for (int at = 1; at < t.edges; at <<= 1) {
+  for (int at = 1; at < t.side; at <<= 1) {
     const int off = ((LPH ? LPH : 1) * at) << p.heads_log2;
     float m2 = __shfl_xor(m, off, kWave), l2 = __shfl_xor(l, off, kWave), acc2[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc2[i] = __shfl_xor(acc[i], off, kWave);
     join<N>(m, l, acc, m2, l2, acc2);
   }
-  if (t.edge != 0 || !t.live) return;
+  if (t.whole) {
+    // All wavefronts of the workgroup are here: theirs are joined to the first one's,
+    // one after the other through one small buffer (LDS is held until the last
+    // wavefront of a workgroup ends, so much of it would keep others out).
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kWave - 1);
+    for (int w = 1; w < kWavesPerBlock; ++w) {
+      if (wave == w) {
+        sh[0][lane] = m;
+        sh[1][lane] = l;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sh[2 + i][lane] = acc[i];
+      }
+      __syncthreads();
+      if (wave == 0) {
+        float a2[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) a2[i] = sh[2 + i][lane];
+        join<N>(m, l, acc, sh[0][lane], sh[1][lane], a2);
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
+  }
+  if (!t.first || !t.live) return;
   if (t.piece >= 0) {
     float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (kPartWide<T, LPH> + 4);
     store_floats<N>(part + t.d0, acc);
@@ -471,6 +505,7 @@ template <typename T, int LPH, bool SHIFTS>
 __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_rows_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
+  __shared__ float sh[2 * N + 1][kWave];
   Task t;
   if (!find_task<T, LPH>(p, p.heads, t)) return;
   const int kv = t.head / p.group;
@@ -508,7 +543,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
       }
     }
   }
-  for (int at = 1; at < t.edges; at <<= 1) {
+  for (int at = 1; at < t.side; at <<= 1) {
     const int off = ((LPH ? LPH : 1) * at) << p.heads_log2;
     rest += __shfl_xor(rest, off, kWave);
 #pragma unroll
@@ -517,8 +552,32 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
       if constexpr (kCorrected<T>) low[i] += __shfl_xor(low[i], off, kWave);
     }
   }
+  if (t.whole) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kWave - 1);
+    for (int w = 1; w < kWavesPerBlock; ++w) {
+      if (wave == w) {
+        sh[0][lane] = rest;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          sh[1 + i][lane] = acc[i];
+          sh[1 + N + i][lane] = low[i];
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+        rest += sh[0][lane];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          acc[i] += sh[1 + i][lane];
+          low[i] += sh[1 + N + i][lane];
+        }
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
+  }
   if (!kCorrected<T>) rest = 0.0f;
-  if (t.edge != 0 || !t.live) return;
+  if (!t.first || !t.live) return;
   if (r == 0.0f) d0 = rest = 0.0f;   // a row of zeros hands nothing on, whatever its gradient holds
   if (t.piece >= 0) {
     float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 4);
@@ -537,6 +596,7 @@ template <typename T, int LPH, bool SHIFTS>
 __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_columns_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
+  __shared__ float sh[2 * N][kWave];
   Task t;
   if (!find_task<T, LPH>(p, p.kv_heads, t)) return;
   float dk[N] = {}, dv[N] = {};
@@ -598,7 +658,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
       }
     }
   }
-  for (int at = 1; at < t.edges; at <<= 1) {
+  for (int at = 1; at < t.side; at <<= 1) {
     const int off = ((LPH ? LPH : 1) * at) << p.heads_log2;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -606,7 +666,29 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
       dv[i] += __shfl_xor(dv[i], off, kWave);
     }
   }
-  if (t.edge != 0 || !t.live) return;
+  if (t.whole) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & (kWave - 1);
+    for (int w = 1; w < kWavesPerBlock; ++w) {
+      if (wave == w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          sh[i][lane] = dk[i];
+          sh[N + i][lane] = dv[i];
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          dk[i] += sh[i][lane];
+          dv[i] += sh[N + i][lane];
+        }
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
+  }
+  if (!t.first || !t.live) return;
   if (t.piece >= 0) {
     float *part = p.part + t.piece * p.part_floats + (int64_t)t.head * (2 * kPartWide<T, LPH> + 4);
     store_floats<N>(part + t.d0, dk);
@@ -725,15 +807,19 @@ static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim
 // 8.5 M 1280 / 1225 / 1138 / 1085.
 static int segment_of(int64_t nnz) { return nnz <= (1 << 18) ? 64 : nnz <= (1 << 20) ? 128 : nnz <= (1 << 22) ? 256 : 512; }
 
-// The second launch costs what about three pieces do one after the other (5 us).
-static bool rows_are_cut(int64_t nnz, int64_t max_row_nnz) {
-  const int64_t uncut = 4 * segment_of(nnz);
-  return nnz > uncut && (max_row_nnz <= 0 || max_row_nnz > uncut || nnz > 0x7fffffff);
+// What becomes of rows longer than that.  Up to 8 times as long (if that is known)
+// they get a workgroup each, whose wavefronts share the row and join in LDS; longer
+// ones are cut into pieces and joined by a second launch (about 5 us).
+enum RowCut { kNone, kWhole, kPieces };
+static RowCut row_cut(int64_t nnz, int64_t max_row_nnz) {
+  const int64_t one = segment_of(nnz);
+  if (nnz <= one || (max_row_nnz > 0 && max_row_nnz <= one && nnz <= 0x7fffffff)) return kNone;
+  return max_row_nnz > 0 && max_row_nnz <= 8 * one && nnz <= 0x7fffffff ? kWhole : kPieces;
 }
 
 static size_t part_bytes(const gcnx_attention *p, int64_t max_row_nnz, int pass) {
   const int64_t nnz = p->a->nnz;
-  if (!rows_are_cut(nnz, max_row_nnz)) return 0;
+  if (row_cut(nnz, max_row_nnz) != kPieces) return 0;
   return align_up((size_t)(2 * ceil_div(nnz, segment_of(nnz))) *
                       part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim) * sizeof(float), 256);
 }
@@ -746,13 +832,13 @@ template <typename T, int LPH, bool SHIFTS>
 static void launch_pass(int pass, const AttnArgs &p, dim3 grid, const AttnArgs &joined, dim3 joins, hipStream_t stream) {
   if (pass == kForward) {
     hipLaunchKernelGGL((attention_forward_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH>), joins, dim3(kBlock), 0, stream, joined);
+    if (p.part_floats) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH>), joins, dim3(kBlock), 0, stream, joined);
   } else if (pass == kBackwardRows) {
     hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, false>), joins, dim3(kBlock), 0, stream, joined);
+    if (p.part_floats) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, false>), joins, dim3(kBlock), 0, stream, joined);
   } else {
     hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
-    if (p.n_pieces) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, true>), joins, dim3(kBlock), 0, stream, joined);
+    if (p.part_floats) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, true>), joins, dim3(kBlock), 0, stream, joined);
   }
 }
 
@@ -865,9 +951,11 @@ static void set_pattern(AttnArgs &g, const gcnx_attention *p, const gcnx_csr *a,
   g.n_rows = a->n_rows;
   g.nnz = a->nnz;
   g.part = part;
-  g.part_floats = part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim);
   g.segment = segment_of(a->nnz);
-  g.n_pieces = rows_are_cut(a->nnz, max_row_nnz) ? 2 * ceil_div(a->nnz, g.segment) : 0;
+  const RowCut cut = row_cut(a->nnz, max_row_nnz);
+  g.whole = cut == kWhole;
+  g.n_pieces = cut == kNone ? 0 : ceil_div(a->nnz, g.segment) * (g.whole ? kWavesPerBlock : 2);
+  g.part_floats = cut == kPieces ? part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim) : 0;
 }
 
 }  // namespace gcnx
@@ -885,8 +973,9 @@ extern "C" int gcnx_attention_forward(const gcnx_attention *p, const int32_t *ch
   if (p->a->n_rows == 0) return GCNX_OK;
   GCNX_REQUIRE(out && stride_ok(out_row) && stride_ok(out_head), GCNX_ERR_INVALID_ARG, "attention: bad output");
   const size_t need = part_bytes(p, p->max_row_nnz, kForward);
-  GCNX_REQUIRE(need == 0 || (chunk_row && ws && ws_bytes >= need), GCNX_ERR_WORKSPACE,
-               "attention: workspace of %zu bytes (and the chunk table) needed, %zu given", need, ws_bytes);
+  GCNX_REQUIRE(need == 0 || (ws && ws_bytes >= need), GCNX_ERR_WORKSPACE, "attention: workspace of %zu bytes needed, %zu given",
+               need, ws_bytes);
+  GCNX_REQUIRE(row_cut(p->a->nnz, p->max_row_nnz) == kNone || chunk_row, GCNX_ERR_INVALID_ARG, "attention: chunk table needed");
   AttnArgs g = common_args(p);
   set_pattern(g, p, p->a, chunk_row, p->mask_index, p->max_row_nnz, kForward, (float *)ws);
   g.o0 = out; g.o0_row = out_row; g.o0_head = out_head;
@@ -919,8 +1008,8 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
   const size_t need = gcnx_attention_backward_workspace_bytes(p, t_max_row_nnz);
   GCNX_REQUIRE(need == 0 || (ws && ws_bytes >= need), GCNX_ERR_WORKSPACE,
                "attention: workspace of %zu bytes needed, %zu given", need, ws_bytes);
-  GCNX_REQUIRE((!rows_are_cut(p->a->nnz, p->max_row_nnz) || chunk_row) &&
-                   (!rows_are_cut(p->a->nnz, t_max_row_nnz) || t_chunk_row), GCNX_ERR_INVALID_ARG,
+  GCNX_REQUIRE((row_cut(p->a->nnz, p->max_row_nnz) == kNone || chunk_row) &&
+                   (row_cut(p->a->nnz, t_max_row_nnz) == kNone || t_chunk_row), GCNX_ERR_INVALID_ARG,
                "attention: chunk table needed");
   const int64_t hd = (int64_t)p->n_heads * p->head_dim, kd = (int64_t)p->n_kv_heads * p->head_dim;
   AttnArgs g = common_args(p);

@@ -47,10 +47,11 @@ def test_attention_descriptors(lib):
     # long rows need a workspace unless the longest row is known to be short
     big = _csr(10, 10, 5000)
     need = lib.gcnx_attention_workspace_bytes(C.byref(_attention(big)))
-    assert need > 0 and lib.gcnx_attention_workspace_bytes(C.byref(_attention(big, max_row_nnz=100))) == 0
+    assert need > 0 and lib.gcnx_attention_workspace_bytes(C.byref(_attention(big, max_row_nnz=512))) == 0
     assert fwd(_attention(big)) == _lib.ERR_WORKSPACE
     assert fwd(_attention(big), ws=PTR, n=need - 1, chunk=PTR) == _lib.ERR_WORKSPACE
-    assert fwd(_attention(big), ws=PTR, n=need) == _lib.ERR_WORKSPACE          # no chunk table
+    assert fwd(_attention(big), ws=PTR, n=need) == _lib.ERR_INVALID_ARG        # no chunk table
+    assert fwd(_attention(big, max_row_nnz=200)) == _lib.ERR_INVALID_ARG       # needed without pieces too
     assert b"attention" in lib.gcnx_last_error()
 
 

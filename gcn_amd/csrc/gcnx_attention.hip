@@ -421,6 +421,7 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
   JoinTask j;
   int slot;
   place_lane<T, LPH>(p, p.heads, blockIdx.y, t, slot);
+  const int head = t.live ? t.head : 0;      // lanes behind the last head read along
   int64_t rows, lasts;
   for (uint64_t left = find_joins(p, rows, lasts); left; left &= left - 1) {
     const int chunk = __builtin_ctzll(left);
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
       float m2[kJoinAhead], l2[kJoinAhead], a2[kJoinAhead][N];
 #pragma unroll
       for (int u = 0; u < kJoinAhead; ++u) {
-        const float *part = j.part(p, c + u * groups) + (int64_t)t.head * (kPartWide<T, LPH> + 4);
+        const float *part = j.part(p, c + u * groups) + (int64_t)head * (kPartWide<T, LPH> + 4);
         m2[u] = part[kPartWide<T, LPH>];
         l2[u] = part[kPartWide<T, LPH> + 1];
         load_floats<N>(part + t.d0, a2[u]);
@@ -713,6 +714,7 @@ __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArg
   JoinTask j;
   int slot;
   place_lane<T, LPH>(p, COLUMNS ? p.kv_heads : p.heads, blockIdx.y, t, slot);
+  const int head = t.live ? t.head : 0;      // lanes behind the last head read along
   int64_t rows, lasts;
   for (uint64_t left = find_joins(p, rows, lasts); left; left &= left - 1) {
     const int chunk = __builtin_ctzll(left);
@@ -724,7 +726,7 @@ __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArg
       float a2[kJoinAhead][N], b2[kJoinAhead][N], rest2[kJoinAhead];
 #pragma unroll
       for (int u = 0; u < kJoinAhead; ++u) {
-        const float *part = j.part(p, c + u * groups) + (int64_t)t.head * (2 * kPartWide<T, LPH> + 4);
+        const float *part = j.part(p, c + u * groups) + (int64_t)head * (2 * kPartWide<T, LPH> + 4);
         load_floats<N>(part + t.d0, a2[u]);
         load_floats<N>(part + kPartWide<T, LPH> + t.d0, b2[u]);
         rest2[u] = COLUMNS ? 0.0f : part[2 * kPartWide<T, LPH>];
@@ -971,7 +973,8 @@ extern "C" int gcnx_attention_forward(const gcnx_attention *p, const int32_t *ch
                                       int64_t out_head, float *stats, void *ws, size_t ws_bytes, void *stream) {
   if (int rc = check(p)) return rc;
   if (p->a->n_rows == 0) return GCNX_OK;
-  GCNX_REQUIRE(out && stride_ok(out_row) && stride_ok(out_head), GCNX_ERR_INVALID_ARG, "attention: bad output");
+  GCNX_REQUIRE(out && stride_ok(out_row) && stride_ok(out_head) && ((uintptr_t)stats & 7) == 0 && ((uintptr_t)ws & 15) == 0,
+               GCNX_ERR_INVALID_ARG, "attention: bad output, or stats or workspace not aligned");
   const size_t need = part_bytes(p, p->max_row_nnz, kForward);
   GCNX_REQUIRE(need == 0 || (ws && ws_bytes >= need), GCNX_ERR_WORKSPACE, "attention: workspace of %zu bytes needed, %zu given",
                need, ws_bytes);
@@ -1003,6 +1006,7 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
                "attention: the mask needs its index in the transpose");
   GCNX_REQUIRE(p->a->n_rows == 0 || (out && dout && stats && stride_ok(out_row) && stride_ok(out_head) && stride_ok(dout_row) && stride_ok(dout_head)),
                GCNX_ERR_INVALID_ARG, "attention: bad output or gradient of it");
+  GCNX_REQUIRE(((uintptr_t)stats & 7) == 0 && ((uintptr_t)ws & 15) == 0, GCNX_ERR_INVALID_ARG, "attention: stats or workspace not aligned");
   GCNX_REQUIRE((dk == nullptr) == (dv == nullptr) && (dq || dk || (p->a->n_rows == 0 && p->a->n_cols == 0)),
                GCNX_ERR_INVALID_ARG, "attention: dq, or dk and dv, or all three");
   const size_t need = gcnx_attention_backward_workspace_bytes(p, t_max_row_nnz);

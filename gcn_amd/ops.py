@@ -553,8 +553,11 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
     strides between head vectors; ``scale`` defaults to ``head_dim ** -0.5``.
     ``mask`` (uint8, in the order of the tuple ``A`` was built from) takes the
     edges with 0 out of the softmax, as a value of -inf does; a row with no edge
-    left gives zeros.  With ``want_stats`` returns ``(out, stats)``, what
-    :func:`attention_bwd` needs.  The attention-weighted sibling of :func:`spmm`
+    left gives zeros.  ``out`` (default: a new tensor) must not share memory with ``k``
+    or ``v``.  With ``want_stats`` returns ``(out, stats)``, what :func:`attention_bwd`
+    needs.  The longest row of ``a`` is looked up at its first use (a host
+    synchronisation; skipped under a stream capture, where it is taken as unknown:
+    the same result but for the order of sums).  The attention-weighted sibling of :func:`spmm`
     (reference gcn/layers.py:219 sums the neighbours with fixed weights)."""
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
@@ -580,7 +583,7 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
     from its ``out`` and ``stats`` (the probabilities are formed again, edge by
     edge).  The gradients of shared key heads are summed over the query heads that
     share them.  ``need_q`` / ``need_kv`` False leaves those gradients out (None).
-    Uses the transpose of ``a`` (built at its first use)."""
+    Uses the transpose of ``a``, built at its first use: before a stream capture."""
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
     dev, dim = q.device, q.shape[2]
@@ -593,6 +596,8 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
         raise ValueError("stats must be what attention(..., want_stats=True) returned")
     if not need_q and not need_kv:
         return None, None, None
+    if a._t is None and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("attention_bwd under a stream capture: build a.transpose() before it")
     at = a.transpose()
     longest = at.max_row_nnz()
     dq = _like(q) if need_q else None
@@ -1089,7 +1094,7 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
     ``w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)``.
     ``state`` is the list's :func:`adamw_state`; ``grads`` (one dtype: float32, bfloat16
     or float16) has one contiguous tensor a param, or None: that param and its state
-    stay as they are.  ``t`` counts from 1 and is either a Python int or a device counter
+    stay as they are.  No two tensors may share memory.  ``t`` counts from 1 and is either a Python int or a device counter
     (read when the kernels run); ``weight_decay`` is a number or one a param.  The
     decoupled many-tensor sibling of :func:`adam_step`."""
     lib = _lib.load()

@@ -528,10 +528,11 @@ int gcnx_gemm_dropout_at_rows_f32(int64_t M, int64_t N, int64_t K, const float *
  * elements, other strides in elements (0 allowed, not negative).  Logits, softmax
  * and sums are fp32, results are rounded once.  Sums have a fixed order: results
  * are bitwise reproducible.
- * Long rows (over 256 .. 2048 edges by the size of the matrix) are cut into pieces
- * joined by a second launch.
- * max_row_nnz, the most edges of a row, says that there are none (0: unknown); it
- * never changes a result beyond that order of sums. */
+ * Rows longer than 64 .. 512 edges (by the size of the matrix) are shared by the
+ * wavefronts of a workgroup, very long ones (8 times that, or where max_row_nnz, the
+ * most edges of a row, is 0 = unknown) cut into pieces joined by a second launch:
+ * both need the matrix's chunk table, the second a workspace (16-byte aligned).  Of a
+ * result that changes only the order of the sums. */
 typedef enum gcnx_dtype { GCNX_F32 = 0, GCNX_BF16 = 1, GCNX_F16 = 2 } gcnx_dtype;
 typedef struct gcnx_attention {
   const gcnx_csr *a;
@@ -549,8 +550,9 @@ typedef struct gcnx_attention {
   const void *v;
   int64_t v_row, v_head;
 } gcnx_attention;
-/* stats (nullable, fp32 [n_rows, n_heads, 2]): the row's largest logit and one over
- * the sum of exp(s - it) (0, 0 for a row of zeros): what the backward needs. */
+/* out must not overlap k or v.  stats (nullable, fp32 [n_rows, n_heads, 2], 8-byte
+ * aligned): the row's largest logit and one over the sum of exp(s - it) (0, 0 for a
+ * row of zeros): what the backward needs. */
 size_t gcnx_attention_workspace_bytes(const gcnx_attention *p);
 int gcnx_attention_forward(const gcnx_attention *p, const int32_t *chunk_row,
                            void *out, int64_t out_row, int64_t out_head,
@@ -595,8 +597,8 @@ typedef struct gcnx_norm_residual {
   const float *res_scale;     /* nullable */
   const float *pre_weight;    /* nullable */
 } gcnx_norm_residual;
-/* y is not written without z, h not without pre_weight.  y may be x, or z.
- * stats (nullable, fp32 [n, 4], 16-byte aligned): what the backward needs. */
+/* y is not written without z, h not without pre_weight; neither may overlap an
+ * operand.  stats (nullable, fp32 [n, 4], 16-byte aligned): what the backward needs. */
 int gcnx_norm_residual_forward(const gcnx_norm_residual *p, void *y, int64_t y_ld,
                                void *h, int64_t h_ld, float *stats, void *stream);
 /* Gradients for dy (nullable: zero) and dh (nullable: zero).  Any result may be

@@ -42,6 +42,8 @@ def test_attention_descriptors(lib):
     noval = _csr()
     noval.val = None
     assert fwd(_attention(noval, use_values=1)) == _lib.ERR_INVALID_ARG
+    assert lib.gcnx_attention_forward(C.byref(_attention(a)), PTR, PTR, 32, 8, PTR + 4, None, 0, None) == _lib.ERR_INVALID_ARG
+    assert fwd(_attention(a), ws=PTR + 8) == _lib.ERR_INVALID_ARG
     # nothing to do is no error, and needs no pointer
     assert fwd(_attention(_csr(0, 5, 0), q=None), out=None) == _lib.OK
     # long rows need a workspace unless the longest row is known to be short

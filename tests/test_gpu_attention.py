@@ -119,6 +119,73 @@ def test_rows_of_many_pieces(env, dtype):
         Case(env, col, row, (700, n_rows), 4, 2, 3, dtype, seed=4).check()
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(5, 5, 8), (3, 1, 20), (11, 11, 65), (1, 1, 2)])
+def test_long_rows_with_idle_lanes(env, heads, kv, dim):
+    """Head counts that leave lanes of a wavefront idle, rows in pieces (the last piece
+    at the end of the workspace) and rows of a workgroup."""
+    rng = np.random.RandomState(dim)
+    for long in (300, 900):
+        row = np.concatenate([rng.randint(0, 4, 50), np.full(long, 4)]).astype(np.int32)
+        col = rng.randint(0, 30, len(row)).astype(np.int32)
+        for dtype in TYPES:
+            Case(env, row, col, (5, 30), heads, kv, dim, dtype, seed=1).check()
+            Case(env, col, row, (30, 5), heads, kv, dim, dtype, seed=2).check()
+
+
+def test_offsets_past_32_bits(env):
+    """Operands of more than 4 GiB, their last rows in use: as columns, then as rows."""
+    torch, ops, dev = env["torch"], env["ops"], env["dev"]
+    n, dim = (1 << 22) + 7, 256
+    rng = np.random.RandomState(5)
+    far = np.concatenate([[0, 1, n - 1, n - 2, n // 2], rng.randint(0, n, 20)]).astype(np.int32)
+    near = rng.randint(0, 3, len(far)).astype(np.int32)
+    small = Case(env, near, np.arange(len(far), dtype=np.int32), (3, len(far)), 1, 1, dim, "float32")
+    want = small.check()
+    at = torch.from_numpy(far.astype(np.int64)).to(dev)
+    first = {int(f): i for i, f in reversed(list(enumerate(far)))}                      # a node drawn twice is one row
+    same = torch.tensor([first[int(f)] for f in far], device=dev)
+    big = lambda t: torch.zeros((n, 1, dim), device=dev).index_copy_(0, at, t[same])
+    a = env["Csr"].from_coo(near, far, np.ones(len(far)), (3, n), dev)
+    k, v = big(small.k), big(small.v)
+    twin = Case(env, near, same.cpu().numpy().astype(np.int32), (3, len(far)), 1, 1, dim, "float32")
+    want = twin.run()
+    out, stats = ops.attention(a, small.q, k, v, want_stats=True)
+    got = (out,) + ops.attention_bwd(a, small.q, k, v, out, stats, small.g)
+    # the same sums, but where duplicates order an edge otherwise
+    close = lambda x, y: torch.allclose(x, y, rtol=1e-4, atol=1e-4)
+    assert close(got[0], want[0]) and close(got[1], want[1])
+    for g, w in zip(got[2:], want[2:]):
+        assert close(g[at], w[same])
+        assert float(g.abs().sum()) == pytest.approx(float(w.abs().sum()), rel=1e-4)     # every other row is zero
+    del k, v, got, out
+    # the far nodes as rows
+    a = env["Csr"].from_coo(far, near, np.ones(len(far)), (n, 3), dev)
+    twin = Case(env, same.cpu().numpy().astype(np.int32), near, (len(far), 3), 1, 1, dim, "float32")
+    want = twin.run()
+    q, g = big(twin.q), big(twin.g)
+    out, stats = ops.attention(a, q, twin.k, twin.v, want_stats=True)
+    got = (out,) + ops.attention_bwd(a, q, twin.k, twin.v, out, stats, g)
+    for x, w in zip(got[:2], want[:2]):
+        assert close(x[at], w[same])
+    for x, w in zip(got[2:], want[2:]):
+        assert close(x, w)
+
+
+def test_no_columns_and_no_rows(env):
+    torch, ops = env["torch"], env["ops"]
+    none = np.zeros(0, np.int32)
+    for shape in ((4, 0), (0, 4), (0, 0)):
+        try:
+            a = env["Csr"].from_coo(none, none, np.zeros(0), shape, env["dev"])
+        except Exception:
+            continue                                        # a matrix that the framework does not make
+        q, k = torch.ones(shape[0], 2, 8, device=env["dev"]), torch.ones(shape[1], 1, 8, device=env["dev"])
+        out, stats = ops.attention(a, q, k, k, want_stats=True)
+        assert out.shape == q.shape and not out.any()
+        dq, dk, dv = ops.attention_bwd(a, q, k, k, out, stats, q)
+        assert not dq.any() and not dk.any() and not dv.any() and dk.shape == k.shape
+
+
 def test_row_length_hint_changes_nothing(env):
     rng = np.random.RandomState(2)
     row, col = _pattern(rng, 400, 300, 3000)              # no row is long; the hint says so, 0 = unknown does not

@@ -54,7 +54,7 @@ class CsrStruct(C.Structure):
 
 class AttentionStruct(C.Structure):
     """Mirror of ``struct gcnx_attention``."""
-    _fields_ = [("a", C.POINTER(CsrStruct)), ("use_values", C.c_int32), ("dtype", C.c_int32),
+    _fields_ = [("a", C.c_void_p), ("use_values", C.c_int32), ("dtype", C.c_int32),
                 ("edge_mask", C.c_void_p), ("mask_index", C.c_void_p), ("max_row_nnz", C.c_int64),
                 ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float),
                 ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),

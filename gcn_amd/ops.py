@@ -471,34 +471,38 @@ def gemm_autograd(a, b, relu=False):
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-def _check_heads(t, name, rows, dim=None, like=None):
-    """The strides of [rows, heads, head_dim] with contiguous head vectors."""
+def _check_heads(t, name, rows, heads, dim, dtype, device):
+    """The strides of ``t`` as [rows, heads, dim] with contiguous head vectors."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError("%s must be a CUDA (ROCm) tensor; gcn_amd has no CPU path" % name)
-    dtype, shape, stride = t.dtype, t.shape, t.stride()
-    if dtype not in _DTYPES:
-        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, dtype))
-    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1 and t.numel()):
-        raise ValueError("%s must be [rows, heads, head_dim] with contiguous head vectors" % name)
-    if shape[0] != rows:
-        raise ValueError("%s has %d rows, the matrix asks for %d" % (name, shape[0], rows))
-    if like is not None and (dtype != like.dtype or t.device != like.device):
-        raise ValueError("%s differs in dtype or device" % name)
-    if dim is not None and shape[2] != dim:
-        raise ValueError("%s has head_dim %d, expected %d" % (name, shape[2], dim))
-    return stride
+    stride = t.stride()
+    if t.shape == (rows, heads, dim) and t.dtype == dtype and t.device == device and (stride[2] == 1 or dim == 1 or not t.numel()):
+        return stride
+    if t.dtype != dtype or t.device != device:
+        raise ValueError("%s differs from q in dtype or device" % name)
+    raise ValueError("%s must be [%d, %d, %d] with contiguous head vectors, got %s with strides %s" %
+                     (name, rows, heads, dim, tuple(t.shape), stride))
 
 
 def _attention_struct(a, q, k, v, scale, use_values, mask):
-    qs = _check_heads(q, "q", a.n_rows)
+    """The descriptor of a call; its tensors are checked."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise RuntimeError("q must be a CUDA (ROCm) tensor; gcn_amd has no CPU path")
+    dtype, dev = q.dtype, q.device
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError("q must be float32, bfloat16 or float16, got %s" % (dtype,))
+    if q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("q and k must be [rows, heads, head_dim]")
     _, heads, dim = q.shape
-    ks = _check_heads(k, "k", a.n_cols, dim, q)
-    vs = _check_heads(v, "v", a.n_cols, dim, q)
-    if q.device != a.device:
-        raise ValueError("the matrix and q live on different devices")
     kv = k.shape[1]
-    if v.shape[1] != kv or kv < 1 or heads < 1 or heads % kv:
-        raise ValueError("%d query heads cannot share %d key and %d value heads" % (heads, kv, v.shape[1]))
+    qs = _check_heads(q, "q", a.n_rows, heads, dim, dtype, dev)
+    ks = _check_heads(k, "k", a.n_cols, kv, dim, dtype, dev)
+    vs = _check_heads(v, "v", a.n_cols, kv, dim, dtype, dev)
+    if dev != a.device:
+        raise ValueError("the matrix and q live on different devices")
+    if kv < 1 or heads < 1 or heads % kv:
+        raise ValueError("%d query heads cannot share %d key heads" % (heads, kv))
     if not 1 <= dim <= 256:
         raise ValueError("head_dim must be 1..256, got %d" % dim)
     mask_ptr = index_ptr = None
@@ -510,7 +514,7 @@ def _attention_struct(a, q, k, v, scale, use_values, mask):
         if a.input_index is not None:
             index_ptr = a.input_index.data_ptr()
     return _lib.AttentionStruct(
-        C.pointer(a._struct), 1 if use_values else 0, _DTYPES[q.dtype], mask_ptr, index_ptr, a.max_row_nnz(), heads, kv, dim,
+        a.struct_address, 1 if use_values else 0, code, mask_ptr, index_ptr, a.max_row_nnz(), heads, kv, dim,
         dim ** -0.5 if scale is None else scale, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
         vs[1])
 
@@ -566,8 +570,8 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
         out = _like(q)
         os = out.stride()
     else:
-        os = _check_heads(out, "out", a.n_rows, q.shape[2], q)
-        if out.shape[1] != q.shape[1] or any(s == 0 and n > 1 for s, n in zip(os, out.shape)):
+        os = _check_heads(out, "out", a.n_rows, q.shape[1], q.shape[2], q.dtype, dev)
+        if any(s == 0 and n > 1 for s, n in zip(os, out.shape)):
             raise ValueError("out must be [n_rows, heads, head_dim] of distinct elements")
     stats = torch.empty((a.n_rows, q.shape[1], 2), dtype=torch.float32, device=dev) if want_stats else None
     with _on(dev):
@@ -586,12 +590,11 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
     Uses the transpose of ``a``, built at its first use: before a stream capture."""
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
-    dev, dim = q.device, q.shape[2]
-    os = _check_heads(out, "out", a.n_rows, dim, q)
-    gs = _check_heads(d_out, "d_out", a.n_rows, dim, q)
-    if out.shape[1] != q.shape[1] or d_out.shape[1] != q.shape[1]:
-        raise ValueError("out and d_out must have the %d heads of q" % q.shape[1])
-    if stats.dtype != torch.float32 or stats.shape != (a.n_rows, q.shape[1], 2) or not stats.is_contiguous() or \
+    dev = q.device
+    n_rows, heads, dim = q.shape
+    os = _check_heads(out, "out", n_rows, heads, dim, q.dtype, dev)
+    gs = _check_heads(d_out, "d_out", n_rows, heads, dim, q.dtype, dev)
+    if stats.dtype != torch.float32 or stats.shape != (n_rows, heads, 2) or not stats.is_contiguous() or \
             stats.device != dev:
         raise ValueError("stats must be what attention(..., want_stats=True) returned")
     if not need_q and not need_kv:

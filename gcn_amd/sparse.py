@@ -85,6 +85,7 @@ class Csr(object):
         self._struct = _lib.CsrStruct(self.n_rows, self.n_cols, self.nnz,
                                       row_ptr.data_ptr(), col_idx.data_ptr(), val.data_ptr(),
                                       int(self.default_spmm_chunk), None)
+        self.struct_address = C.addressof(self._struct)
         lib = _lib.load()
         n_chunks = lib.gcnx_spmm_num_chunks(self.nnz)
         self.chunk_row = torch.empty(n_chunks + 1, dtype=torch.int32, device=self.device)

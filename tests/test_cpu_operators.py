@@ -24,7 +24,9 @@ def _attention(a, **kw):
     f = dict(use_values=0, dtype=_lib.F32, edge_mask=None, mask_index=None, max_row_nnz=0, n_heads=4, n_kv_heads=2, head_dim=8, scale=1.0,
              q=PTR, q_row=32, q_head=8, k=PTR, k_row=16, k_head=8, v=PTR, v_row=16, v_head=8)
     f.update(kw)
-    return _lib.AttentionStruct(a=C.pointer(a), **f)
+    p = _lib.AttentionStruct(a=C.addressof(a), **f)
+    p.matrix = a                     # kept alive
+    return p
 
 
 def test_attention_descriptors(lib):

@@ -383,9 +383,17 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forwa
 
 // Joining the pieces of cut rows: those that begin in one of kJoinChunks chunks, a
 // tile of heads of them, by a workgroup.  A row's pieces are slot 1 of the chunk that
-// it begins in and slot 0 of the chunks after it; they are dealt to groups of lanes, kJoinAhead read at a time, each group joins its own in order, then groups
-// are joined by exchanges in the wavefront and through LDS: a fixed tree.
-constexpr int kJoinChunks = 4;
+// it begins in and slot 0 of the chunks after it.  Rows of up to kJoinWave pieces are
+// dealt to the wavefronts, longer ones are the whole workgroup's.  The pieces of a row
+// are dealt to groups of lanes, kJoinAhead read at a time; each group joins its own in
+// order, then groups are joined by exchanges in the wavefront and (for the workgroup's
+// rows) through LDS: a fixed tree.
+// Latency bounds it.  us of the backward pass's join, every row the workgroup's and 4
+// chunks -> this: 8.5 M edges of 2^19 rows 40 -> 25 (columns 29 -> 21), 0.9 M edges of
+// heads 8 on 2 x 64 31 -> 28 (17 -> 10), 2^20 edges of 3 rows 23 -> 17.  16 chunks: the
+// same within 2 us; kJoinWave 32: the same.
+constexpr int kJoinChunks = 8;
+constexpr int kJoinWave = 16;
 constexpr int kJoinAhead = 4;
 
 struct JoinTask {
@@ -397,7 +405,7 @@ struct JoinTask {
 
 // Which of the workgroup's chunks have a cut row begin in them, a lane a chunk; row
 // and last chunk of the lane's.
-__device__ __forceinline__ uint64_t find_joins(const AttnArgs &p, int64_t &row, int64_t &last) {
+__device__ __forceinline__ uint64_t find_joins(const AttnArgs &p, int64_t &row, int64_t &last, uint64_t &small) {
   const int lane = threadIdx.x & (kWave - 1);
   const int64_t first = ((int64_t)blockIdx.x * kJoinChunks + lane) * p.segment, next = first + p.segment;
   bool found = false;
@@ -408,13 +416,14 @@ __device__ __forceinline__ uint64_t find_joins(const AttnArgs &p, int64_t &row, 
     last = (end - 1) / p.segment;
     found = beg >= first && beg < next && end - beg > p.segment;
   }
+  small = __ballot(found && last - (next / p.segment - 1) < kJoinWave);
   return __ballot(found);
 }
 
 template <typename T, int LPH>
 __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N, L = LPH ? LPH : 1;
-  const int span = L << p.heads_log2, groups = kBlock / span;     // lanes of a group
+  const int span = L << p.heads_log2;        // lanes of a group
   __shared__ float sh[kWavesPerBlock][kWave][N + 2];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   Task t;
@@ -423,13 +432,15 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
   place_lane<T, LPH>(p, p.heads, blockIdx.y, t, slot);
   const int head = t.live ? t.head : 0;      // lanes behind the last head read along
   int64_t rows, lasts;
-  for (uint64_t left = find_joins(p, rows, lasts); left; left &= left - 1) {
-    const int chunk = __builtin_ctzll(left);
+  uint64_t small;
+  const uint64_t found = find_joins(p, rows, lasts, small);
+  const auto join_row = [&](int chunk, bool block) {
+    const int groups = (block ? kBlock : kWave) / span, group = (block ? threadIdx.x : lane) / span;
     t.row = __shfl(rows, chunk, kWave);
     j.first = (int64_t)blockIdx.x * kJoinChunks + chunk;
     j.last = __shfl(lasts, chunk, kWave);
     float m = -__builtin_inff(), l = 0.0f, acc[N] = {};
-    for (int64_t c = j.first + threadIdx.x / span; c <= j.last; c += kJoinAhead * groups) {
+    for (int64_t c = j.first + group; c <= j.last; c += kJoinAhead * groups) {
       float m2[kJoinAhead], l2[kJoinAhead], a2[kJoinAhead][N];
 #pragma unroll
       for (int u = 0; u < kJoinAhead; ++u) {
@@ -448,25 +459,31 @@ __global__ __launch_bounds__(kBlock) void attention_forward_join_kernel(AttnArgs
       for (int i = 0; i < N; ++i) a2[i] = __shfl_xor(acc[i], off, kWave);
       join<N>(m, l, acc, m2, l2, a2);
     }
-    __syncthreads();
-    if (lane < span) {
-      sh[wave][lane][0] = m;
-      sh[wave][lane][1] = l;
+    if (block) {
+      __syncthreads();
+      if (lane < span) {
+        sh[wave][lane][0] = m;
+        sh[wave][lane][1] = l;
 #pragma unroll
-      for (int i = 0; i < N; ++i) sh[wave][lane][2 + i] = acc[i];
-    }
-    __syncthreads();
-    if (threadIdx.x < span && t.live) {
-#pragma unroll
-      for (int w = 1; w < kWavesPerBlock; ++w) {
-        float a2[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) a2[i] = sh[w][lane][2 + i];
-        join<N>(m, l, acc, sh[w][lane][0], sh[w][lane][1], a2);
+        for (int i = 0; i < N; ++i) sh[wave][lane][2 + i] = acc[i];
       }
-      finish_forward<T, LPH, N>(p, t, m, l, acc);
+      __syncthreads();
+      if (wave != 0) return;
+      if (lane < span)
+#pragma unroll
+        for (int w = 1; w < kWavesPerBlock; ++w) {
+          float a2[N];
+#pragma unroll
+          for (int i = 0; i < N; ++i) a2[i] = sh[w][lane][2 + i];
+          join<N>(m, l, acc, sh[w][lane][0], sh[w][lane][1], a2);
+        }
     }
-  }
+    if (lane < span && t.live) finish_forward<T, LPH, N>(p, t, m, l, acc);
+  };
+  int turn = 0;
+  for (uint64_t left = small; left; left &= left - 1)
+    if (turn++ % kWavesPerBlock == wave) join_row(__builtin_ctzll(left), false);
+  for (uint64_t left = found & ~small; left; left &= left - 1) join_row(__builtin_ctzll(left), true);
 }
 
 // Row pass of the backward: delta, dq.  Writes m, r, delta side by side for the
@@ -707,7 +724,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
 template <typename T, int LPH, bool COLUMNS>
 __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N, L = LPH ? LPH : 1;
-  const int span = L << p.heads_log2, groups = kBlock / span;     // lanes of a group
+  const int span = L << p.heads_log2;        // lanes of a group
   __shared__ float sh[kWavesPerBlock][kWave][2 * N + 1];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   Task t;
@@ -716,13 +733,15 @@ __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArg
   place_lane<T, LPH>(p, COLUMNS ? p.kv_heads : p.heads, blockIdx.y, t, slot);
   const int head = t.live ? t.head : 0;      // lanes behind the last head read along
   int64_t rows, lasts;
-  for (uint64_t left = find_joins(p, rows, lasts); left; left &= left - 1) {
-    const int chunk = __builtin_ctzll(left);
+  uint64_t small;
+  const uint64_t found = find_joins(p, rows, lasts, small);
+  const auto join_row = [&](int chunk, bool block) {
+    const int groups = (block ? kBlock : kWave) / span, group = (block ? threadIdx.x : lane) / span;
     t.row = __shfl(rows, chunk, kWave);
     j.first = (int64_t)blockIdx.x * kJoinChunks + chunk;
     j.last = __shfl(lasts, chunk, kWave);
     float a[N] = {}, b[N] = {}, rest = 0.0f;
-    for (int64_t c = j.first + threadIdx.x / span; c <= j.last; c += kJoinAhead * groups) {
+    for (int64_t c = j.first + group; c <= j.last; c += kJoinAhead * groups) {
       float a2[kJoinAhead][N], b2[kJoinAhead][N], rest2[kJoinAhead];
 #pragma unroll
       for (int u = 0; u < kJoinAhead; ++u) {
@@ -750,39 +769,46 @@ __global__ __launch_bounds__(kBlock) void attention_backward_join_kernel(AttnArg
       }
       rest += __shfl_xor(rest, off, kWave);
     }
-    __syncthreads();
-    if (lane < span) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        sh[wave][lane][i] = a[i];
-        sh[wave][lane][N + i] = b[i];
-      }
-      sh[wave][lane][2 * N] = rest;
-    }
     float m = 0.0f, r = 0.0f, d0 = 0.0f;
-    if (!COLUMNS && wave == 0) load_row<T, LPH>(p, t, m, r, d0);
-    __syncthreads();
-    if (threadIdx.x < span && t.live) {
-#pragma unroll
-      for (int w = 1; w < kWavesPerBlock; ++w) {
+    if (!COLUMNS && (!block || wave == 0)) load_row<T, LPH>(p, t, m, r, d0);
+    if (block) {
+      __syncthreads();
+      if (lane < span) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          a[i] += sh[w][lane][i];
-          b[i] += sh[w][lane][N + i];
+          sh[wave][lane][i] = a[i];
+          sh[wave][lane][N + i] = b[i];
         }
-        rest += sh[w][lane][2 * N];
+        sh[wave][lane][2 * N] = rest;
       }
-      if constexpr (COLUMNS) {
+      __syncthreads();
+      if (wave != 0) return;
+      if (lane < span)
 #pragma unroll
-        for (int i = 0; i < N; ++i) a[i] *= p.scale;
-        store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, a);
-        store_piece<T, LPH == 0>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, p.dim, b);
-      } else {
-        if (r == 0.0f) d0 = rest = 0.0f;
-        finish_rows<T, LPH, N>(p, t, m, r, d0, rest, a, b);
-      }
+        for (int w = 1; w < kWavesPerBlock; ++w) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            a[i] += sh[w][lane][i];
+            b[i] += sh[w][lane][N + i];
+          }
+          rest += sh[w][lane][2 * N];
+        }
     }
-  }
+    if (lane >= span || !t.live) return;
+    if constexpr (COLUMNS) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] *= p.scale;
+      store_piece<T, LPH == 0>((T *)p.o0 + t.row * p.o0_row + t.head * p.o0_head + t.d0, p.dim, a);
+      store_piece<T, LPH == 0>((T *)p.o1 + t.row * p.o1_row + t.head * p.o1_head + t.d0, p.dim, b);
+    } else {
+      if (r == 0.0f) d0 = rest = 0.0f;
+      finish_rows<T, LPH, N>(p, t, m, r, d0, rest, a, b);
+    }
+  };
+  int turn = 0;
+  for (uint64_t left = small; left; left &= left - 1)
+    if (turn++ % kWavesPerBlock == wave) join_row(__builtin_ctzll(left), false);
+  for (uint64_t left = found & ~small; left; left &= left - 1) join_row(__builtin_ctzll(left), true);
 }
 
 // ------------------------------------------------------------------ host side
@@ -804,25 +830,31 @@ static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim
 
 // Edges a wavefront takes of one row at most: a long row is the last to end where
 // there are few rows, and pieces cost partial results where there are many.
-// Forward and its join, us, at 64 / 128 / 256 / 512 (8 x 32 and 8 on 2 x 64 heads):
-// 0.1 M edges 29 / 35 / 49 / 81, 0.9 M 255 / 273 / 310 / 363, 1 M 125 / 121 / 121 / 139,
-// 8.5 M 1280 / 1225 / 1138 / 1085.
-static int segment_of(int64_t nnz) { return nnz <= (1 << 18) ? 64 : nnz <= (1 << 20) ? 128 : nnz <= (1 << 22) ? 256 : 512; }
+// The forward pass with its join, us, at 64 / 128 / 256 / 512 (heads of 8 x 16, 8 on
+// 2 x 64, 8 x 32, 8 x 32): 0.1 M edges 24 / 26 / 28 / 39, 0.9 M 177 / 181 / 220 / 256,
+// 1 M 108 / 109 / 109 / 138, 8.5 M 1130 / 1096 / 1046 / 1057.
+// Where rows average over 1024 pieces their joins are what takes long, and pieces get
+// longer: 2^20 edges of 3 rows 133 / 111 / 95 / 115.
+static int segment_of(int64_t nnz, int64_t n_rows) {
+  int one = nnz <= (1 << 20) ? 64 : nnz <= (1 << 22) ? 128 : nnz <= (1 << 24) ? 256 : 512;
+  while (one < 512 && n_rows * 1024 * one < nnz) one *= 2;
+  return one;
+}
 
 // What becomes of rows longer than that.  Up to 8 times as long (if that is known)
 // they get a workgroup each, whose wavefronts share the row and join in LDS; longer
 // ones are cut into pieces and joined by a second launch (about 5 us).
 enum RowCut { kNone, kWhole, kPieces };
-static RowCut row_cut(int64_t nnz, int64_t max_row_nnz) {
-  const int64_t one = segment_of(nnz);
+static RowCut row_cut(int64_t nnz, int64_t n_rows, int64_t max_row_nnz) {
+  const int64_t one = segment_of(nnz, n_rows);
   if (nnz <= one || (max_row_nnz > 0 && max_row_nnz <= one && nnz <= 0x7fffffff)) return kNone;
   return max_row_nnz > 0 && max_row_nnz <= 8 * one && nnz <= 0x7fffffff ? kWhole : kPieces;
 }
 
 static size_t part_bytes(const gcnx_attention *p, int64_t max_row_nnz, int pass) {
-  const int64_t nnz = p->a->nnz;
-  if (row_cut(nnz, max_row_nnz) != kPieces) return 0;
-  return align_up((size_t)(2 * ceil_div(nnz, segment_of(nnz))) *
+  const int64_t nnz = p->a->nnz, n_rows = pass == kBackwardColumns ? p->a->n_cols : p->a->n_rows;
+  if (row_cut(nnz, n_rows, max_row_nnz) != kPieces) return 0;
+  return align_up((size_t)(2 * ceil_div(nnz, segment_of(nnz, n_rows))) *
                       part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim) * sizeof(float), 256);
 }
 
@@ -953,8 +985,8 @@ static void set_pattern(AttnArgs &g, const gcnx_attention *p, const gcnx_csr *a,
   g.n_rows = a->n_rows;
   g.nnz = a->nnz;
   g.part = part;
-  g.segment = segment_of(a->nnz);
-  const RowCut cut = row_cut(a->nnz, max_row_nnz);
+  g.segment = segment_of(a->nnz, a->n_rows);
+  const RowCut cut = row_cut(a->nnz, a->n_rows, max_row_nnz);
   g.whole = cut == kWhole;
   g.n_pieces = cut == kNone ? 0 : ceil_div(a->nnz, g.segment) * (g.whole ? kWavesPerBlock : 2);
   g.part_floats = cut == kPieces ? part_floats(pass, p->dtype, p->n_heads, p->n_kv_heads, p->head_dim) : 0;
@@ -978,7 +1010,7 @@ extern "C" int gcnx_attention_forward(const gcnx_attention *p, const int32_t *ch
   const size_t need = part_bytes(p, p->max_row_nnz, kForward);
   GCNX_REQUIRE(need == 0 || (ws && ws_bytes >= need), GCNX_ERR_WORKSPACE, "attention: workspace of %zu bytes needed, %zu given",
                need, ws_bytes);
-  GCNX_REQUIRE(row_cut(p->a->nnz, p->max_row_nnz) == kNone || chunk_row, GCNX_ERR_INVALID_ARG, "attention: chunk table needed");
+  GCNX_REQUIRE(row_cut(p->a->nnz, p->a->n_rows, p->max_row_nnz) == kNone || chunk_row, GCNX_ERR_INVALID_ARG, "attention: chunk table needed");
   AttnArgs g = common_args(p);
   set_pattern(g, p, p->a, chunk_row, p->mask_index, p->max_row_nnz, kForward, (float *)ws);
   g.o0 = out; g.o0_row = out_row; g.o0_head = out_head;
@@ -1012,8 +1044,8 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
   const size_t need = gcnx_attention_backward_workspace_bytes(p, t_max_row_nnz);
   GCNX_REQUIRE(need == 0 || (ws && ws_bytes >= need), GCNX_ERR_WORKSPACE,
                "attention: workspace of %zu bytes needed, %zu given", need, ws_bytes);
-  GCNX_REQUIRE((row_cut(p->a->nnz, p->max_row_nnz) == kNone || chunk_row) &&
-                   (row_cut(p->a->nnz, t_max_row_nnz) == kNone || t_chunk_row), GCNX_ERR_INVALID_ARG,
+  GCNX_REQUIRE((row_cut(p->a->nnz, p->a->n_rows, p->max_row_nnz) == kNone || chunk_row) &&
+                   (row_cut(p->a->nnz, p->a->n_cols, t_max_row_nnz) == kNone || t_chunk_row), GCNX_ERR_INVALID_ARG,
                "attention: chunk table needed");
   const int64_t hd = (int64_t)p->n_heads * p->head_dim, kd = (int64_t)p->n_kv_heads * p->head_dim;
   AttnArgs g = common_args(p);

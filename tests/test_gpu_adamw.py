@@ -301,6 +301,10 @@ def test_refusals(env):
         ops.adamw_step([a, b], [a.double(), b.double()], st, 0.1, 1)
     with pytest.raises(ValueError):
         ops.adamw_step([a, a.view(8)], [a, a], ops.adamw_state([a, a]), 0.1, 1)
+    flat = torch.zeros(17, device=dev)
+    with pytest.raises(ValueError):
+        ops.adamw_step([flat[8:16], flat[:9]], [a, b], st, 0.1, 1)
+    ops.adamw_step([flat[9:], flat[:9]], [a, b], st, 0.1, 1)                    # side by side
     with pytest.raises(ValueError):
         ops.adamw_step([a, b], [a, b], st, 0.1, torch.zeros(1, device=dev))
     from gcn_amd._lib import GcnxError

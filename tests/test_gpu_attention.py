@@ -337,6 +337,12 @@ def test_autograd(env):
     one = c.q[:1].clone().requires_grad_(True)
     ops.attention_autograd(c.a, one.expand(40, -1, -1), c.k, c.v).sum().backward()
     assert one.grad.shape == (1, 4, 8) and torch.isfinite(one.grad).all()
+    # a mask changed between the two passes is noticed
+    mask = torch.ones(c.a.nnz, dtype=torch.uint8, device=env["dev"])
+    out = ops.attention_autograd(c.a, leaves[0], c.k, c.v, mask=mask)
+    mask[0] = 0
+    with pytest.raises(RuntimeError):
+        out.backward(c.g)
     # only what is asked for
     out, stats = ops.attention(c.a, c.q, c.k, c.v, want_stats=True)
     dq, dk, dv = ops.attention_bwd(c.a, c.q, c.k, c.v, out, stats, c.g, need_kv=False)

@@ -63,7 +63,7 @@ constexpr int kBackwardEdges = 1;
 // nothing is spilled for it.  (Column pass at 2^19 nodes: 1284 us against 1525 with
 // the 5 that the compiler chooses.)
 template <int LPH, bool SHIFTS>
-constexpr int kWaves = SHIFTS || LPH == 0 || LPH >= 32 ? 6 : 8;
+constexpr int kWaves = SHIFTS && LPH == 0 ? 5 : SHIFTS || LPH == 0 || LPH >= 32 ? 6 : 8;
 
 struct AttnArgs {
   // pattern walked by this pass (the matrix, or its transpose)

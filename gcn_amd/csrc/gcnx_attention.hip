@@ -907,12 +907,14 @@ static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   p.tiles_log2 = p.tiles <= 8 && (p.tiles & (p.tiles - 1)) == 0 ? log2_ceil(p.tiles) : -1;
   int64_t blocks = ceil_div(p.n_pieces + ceil_div(p.n_rows, (int64_t)1 << p.row_log2), kWavesPerBlock);
   blocks = p.tiles_log2 >= 0 ? ceil_div(blocks, 8 >> p.tiles_log2) * 8 : blocks * p.tiles;
-  GCNX_REQUIRE(blocks <= 0x7fffffff && p.n_pieces / 2 <= 0x7fffffff, GCNX_ERR_UNSUPPORTED, "attention: too many rows for one launch");
   const dim3 grid((unsigned)blocks);
   // few rows of many pieces: a workgroup per head instead of one for a tile of them
   AttnArgs joined = p;
   if (p.n_pieces / 2 / p.n_rows >= 16) joined.heads_log2 = 0;
-  const dim3 joins((unsigned)ceil_div(p.n_pieces / 2, kJoinChunks), (unsigned)ceil_div(heads, (int64_t)1 << joined.heads_log2));
+  const int64_t join_blocks = ceil_div(p.n_pieces / 2, kJoinChunks), join_tiles = ceil_div(heads, (int64_t)1 << joined.heads_log2);
+  GCNX_REQUIRE(blocks < (1ll << 32) / kBlock && join_blocks < (1ll << 32) / kBlock, GCNX_ERR_UNSUPPORTED,
+               "attention: %lld rows, %lld nonzeros and %d heads are too many for one launch", (long long)p.n_rows, (long long)p.nnz, heads);
+  const dim3 joins((unsigned)join_blocks, (unsigned)join_tiles);
   if (p.val || p.mask) launch_pass<T, LPH, true>(pass, p, grid, joined, joins, stream);
   else launch_pass<T, LPH, false>(pass, p, grid, joined, joins, stream);
   GCNX_CHECK_LAUNCH();

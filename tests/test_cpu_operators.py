@@ -48,6 +48,8 @@ def test_attention_descriptors(lib):
     assert fwd(_attention(a), ws=PTR + 8) == _lib.ERR_INVALID_ARG
     # nothing to do is no error, and needs no pointer
     assert fwd(_attention(_csr(0, 5, 0), q=None), out=None) == _lib.OK
+    # more workgroups than a launch has: refused on the host
+    assert fwd(_attention(_csr((1 << 31) - 2, 5, 6), n_heads=64, n_kv_heads=64, head_dim=256)) == _lib.ERR_UNSUPPORTED
     # long rows need a workspace unless the longest row is known to be short
     big = _csr(10, 10, 5000)
     need = lib.gcnx_attention_workspace_bytes(C.byref(_attention(big)))

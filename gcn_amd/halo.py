@@ -40,7 +40,7 @@ def device_halo_plan(a_local, row_begin, n_loc):
     n_halo = int(n_need.value)
     need = need[:n_halo].clone()
     csr = Csr(a_local.n_rows, int(n_loc) + n_halo, a_local.row_ptr, col_new, a_local.val,
-              a_local.input_index)
+              a_local.input_index, a_local.input_nnz)
     return csr, need
 
 

@@ -68,7 +68,7 @@ def _transform(run, x, w, keep, key, relu):
         if keep < 1.0:
             if mask is not None:
                 raise NotImplementedError("sparse dropout applied twice to one tensor")
-            mask = run.dropout_mask(key, x.csr.nnz, keep)
+            mask = run.dropout_mask(key, x.csr.input_nnz, keep)
             scale = scale / keep
         return ops.spmm_autograd(x.csr, w, mask, scale, relu)
     if keep < 1.0:

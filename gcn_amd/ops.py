@@ -70,8 +70,7 @@ def spmm(a, b, out=None, alpha=1.0, beta=0.0, mask=None, mask_scale=1.0, relu=Fa
             raise ValueError("out has shape %s, expected %s" % (tuple(out.shape), (a.n_rows, width)))
     midx = None
     if mask is not None:
-        if mask.dtype != torch.uint8 or mask.numel() != a.nnz or mask.device != a.device:
-            raise ValueError("mask must be uint8 with one byte per nonzero on A's device")
+        a.check_mask(mask)
         midx = a.input_index
     drop = None
     if dropout is not None and dropout[0] < 1.0:
@@ -507,9 +506,7 @@ def _attention_struct(a, q, k, v, scale, use_values, mask):
         raise ValueError("head_dim must be 1..256, got %d" % dim)
     mask_ptr = index_ptr = None
     if mask is not None:
-        if mask.dtype != torch.uint8 or mask.dim() != 1 or mask.numel() != a.nnz or not mask.is_contiguous() or \
-                mask.device != a.device:
-            raise ValueError("mask must be contiguous uint8 with one byte per nonzero on A's device")
+        a.check_mask(mask)
         mask_ptr = mask.data_ptr()
         if a.input_index is not None:
             index_ptr = a.input_index.data_ptr()

@@ -62,7 +62,9 @@ class Csr(object):
     ``val`` fp32 [nnz]; rows ordered by column, duplicates in input order.
     ``input_index[slot]`` is the position of the entry in the tuple the matrix
     was built from (dropout masks are drawn in that order,
-    reference gcn/layers.py:21-27).  ``spmm_chunk`` is the per-matrix dispatch
+    reference gcn/layers.py:21-27); that tuple has ``input_nnz`` entries, more than
+    ``nnz`` where the matrix holds a part of them (:meth:`filter_columns`).  Without
+    an ``input_index`` the order is that of the nonzeros.  ``spmm_chunk`` is the per-matrix dispatch
     hint of the SpMM entry points (0: the library chooses; 64..512: chunk
     kernels with that many nonzeros per wavefront); new matrices take the class
     attribute ``default_spmm_chunk``, which the kernel tests override to run
@@ -70,7 +72,7 @@ class Csr(object):
 
     default_spmm_chunk = 0
 
-    def __init__(self, n_rows, n_cols, row_ptr, col_idx, val, input_index=None):
+    def __init__(self, n_rows, n_cols, row_ptr, col_idx, val, input_index=None, input_nnz=None):
         self.n_rows = int(n_rows)
         self.n_cols = int(n_cols)
         self.nnz = int(col_idx.numel())
@@ -78,6 +80,7 @@ class Csr(object):
         self.col_idx = col_idx
         self.val = val
         self.input_index = input_index
+        self.input_nnz = self.nnz if input_index is None or input_nnz is None else int(input_nnz)
         self.device = row_ptr.device
         self._t = None
         self._max_row = None
@@ -115,6 +118,12 @@ class Csr(object):
                 return 0
             self._max_row = int((self.row_ptr[1:] - self.row_ptr[:-1]).max().item()) if self.n_rows else 0
         return self._max_row
+
+    def check_mask(self, mask):
+        """Raises unless ``mask`` is one contiguous byte per entry of the tuple the
+        matrix was built from, on its device."""
+        if mask.dtype != torch.uint8 or mask.numel() != self.input_nnz or not mask.is_contiguous() or mask.device != self.device:
+            raise ValueError("mask must be contiguous uint8 with one byte per entry of the tuple (%d) on A's device" % self.input_nnz)
 
     # -------------------------------------------------------------- cache hint
     def column_degrees(self):
@@ -181,7 +190,7 @@ class Csr(object):
                                                         _ptr(val), _ptr(src), _stream()))
         idx = self.input_index[src] if self.input_index is not None else None
         del ws
-        return Csr(self.n_rows, self.n_cols, row_ptr, col, val, idx)
+        return Csr(self.n_rows, self.n_cols, row_ptr, col, val, idx, self.input_nnz)
 
     def compact_rows(self):
         """``(sub, rows)``: the matrix without its empty rows (``sub`` shares the
@@ -191,7 +200,7 @@ class Csr(object):
         deg = self.row_ptr[1:] - self.row_ptr[:-1]
         rows = torch.nonzero(deg > 0).view(-1)
         row_ptr = torch.cat([self.row_ptr[rows], self.row_ptr[-1:]]).contiguous()
-        sub = Csr(int(rows.numel()), self.n_cols, row_ptr, self.col_idx, self.val, self.input_index)
+        sub = Csr(int(rows.numel()), self.n_cols, row_ptr, self.col_idx, self.val, self.input_index, self.input_nnz)
         return sub, rows.to(torch.int32).contiguous()
 
     def keep_rows(self, rows):
@@ -207,7 +216,7 @@ class Csr(object):
         if kept != self.nnz:
             raise ValueError("keep_rows: a row that is left out holds nonzeros (%d of %d kept)" % (kept, self.nnz))
         row_ptr = torch.cat([self.row_ptr[r], self.row_ptr[-1:]]).contiguous()
-        return Csr(int(r.numel()), self.n_cols, row_ptr, self.col_idx, self.val, self.input_index)
+        return Csr(int(r.numel()), self.n_cols, row_ptr, self.col_idx, self.val, self.input_index, self.input_nnz)
 
     # ---------------------------------------------------------------- builders
     @classmethod
@@ -295,7 +304,7 @@ class Csr(object):
         if not cache:
             return Csr(self.n_cols, self.n_rows, t_row_ptr, t_col_idx, t_val, None)
         idx = self.input_index[t_perm] if self.input_index is not None else t_perm
-        t = Csr(self.n_cols, self.n_rows, t_row_ptr, t_col_idx, t_val, idx)
+        t = Csr(self.n_cols, self.n_rows, t_row_ptr, t_col_idx, t_val, idx, self.input_nnz)
         t._t = self
         self._t = t
         return t

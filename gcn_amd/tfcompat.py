@@ -428,7 +428,7 @@ def sparse_retain_scaled(x, keep_prob, seed_key):
             return xv
         if xv.mask is not None:
             raise NotImplementedError("sparse dropout applied twice to one tensor")
-        mask = run.dropout_mask(seed_key, xv.csr.nnz, keep)
+        mask = run.dropout_mask(seed_key, xv.csr.input_nnz, keep)
         return SparseValue(xv.csr, mask, xv.scale / keep, xv.source)
     return Node(fn, (x, keep_prob))
 

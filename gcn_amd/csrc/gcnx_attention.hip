@@ -61,9 +61,10 @@ constexpr int kBackwardEdges = 1;
 
 // Wavefronts a SIMD that the registers have to leave room for: 8 (64 registers) where
 // nothing is spilled for it.  (Column pass at 2^19 nodes: 1284 us against 1525 with
-// the 5 that the compiler chooses.)
-template <int LPH, bool SHIFTS>
-constexpr int kWaves = SHIFTS && LPH == 0 ? 5 : SHIFTS || LPH == 0 || LPH >= 32 ? 6 : 8;
+// the 5 that the compiler chooses.)  The backward passes of ragged heads hold four
+// words more.
+template <int LPH, bool SHIFTS, bool RAGGED = false>
+constexpr int kWaves = SHIFTS && LPH == 0 ? 5 : SHIFTS || LPH == 0 || LPH >= 32 ? 6 : RAGGED ? 7 : 8;
 
 struct AttnArgs {
   // pattern walked by this pass (the matrix, or its transpose)
@@ -299,7 +300,7 @@ __device__ __forceinline__ void finish_forward(const AttnArgs &p, const Task &t,
 template <typename T, int LPH>
 constexpr int kPartWide = (LPH ? LPH : 1) * Piece<T>::N;
 
-template <typename T, int LPH, bool SHIFTS>
+template <typename T, int LPH, bool SHIFTS, bool RAGGED>
 __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forward_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
@@ -308,6 +309,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forwa
   if (!find_task<T, LPH>(p, p.heads, t)) return;
   const int kv = t.head / p.group;
   const raw q = load_own<T, LPH>(p, t, p.q, p.q_row, p.q_head);
+  const Counted<T, RAGGED> counted(t.skip);
   float acc[N] = {}, m = -__builtin_inff(), l = 0.0f;
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (t.count) {
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forwa
       float top = m;
 #pragma unroll
       for (int u = 0; u < kForwardEdges; ++u) {
-        const float d = group_sum<LPH>(dot_piece<T>(q, k[u]));
+        const float d = group_sum<LPH>(dot_piece<T>(q, counted.of(k[u])));
         s[u] = on[u] ? fmaf(d, p.scale, s[u]) : -__builtin_inff();
         top = fmaxf(top, s[u]);
       }
@@ -529,8 +531,8 @@ __device__ __forceinline__ typename Piece<T>::raw load_row(const AttnArgs &p, co
   return g;
 }
 
-template <typename T, int LPH, bool SHIFTS>
-__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_rows_kernel(AttnArgs p) {
+template <typename T, int LPH, bool SHIFTS, bool RAGGED>
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attention_backward_rows_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   __shared__ float sh[2 * N + 1][kWave];
@@ -539,6 +541,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
   const int kv = t.head / p.group;
   float acc[N] = {}, low[N] = {}, m, r, d0, rest = 0.0f;
   const raw q = load_own<T, LPH>(p, t, p.q, p.q_row, p.q_head), g = load_row<T, LPH>(p, t, m, r, d0);
+  const Counted<T, RAGGED> counted(t.skip);
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (!kCorrected<T> && !p.o0) t.count = 0;        // delta alone is asked for
   if (t.count) {
@@ -559,7 +562,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
       read_ahead_fence();
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
-        const float s = group_sum<LPH>(dot_piece<T>(q, k[u])), d = group_sum<LPH>(dot_piece<T>(g, v[u]));
+        const float s = group_sum<LPH>(dot_piece<T>(q, counted.of(k[u]))), d = group_sum<LPH>(dot_piece<T>(g, counted.of(v[u])));
         const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r : 0.0f;
         const float ds = on[u] ? w * (d - d0) : 0.0f;
         rest += ds;
@@ -620,8 +623,8 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
 // Column pass: a row of the transpose is a column j of the pattern.  The lanes own
 // the key heads; the edges of the column are walked once per query head that
 // shares the key head, as count * group items.
-template <typename T, int LPH, bool SHIFTS>
-__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_columns_kernel(AttnArgs p) {
+template <typename T, int LPH, bool SHIFTS, bool RAGGED>
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attention_backward_columns_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   __shared__ float sh[2 * N][kWave];
@@ -629,6 +632,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
   if (!find_task<T, LPH>(p, p.kv_heads, t)) return;
   float dk[N] = {}, dv[N] = {};
   const raw k = load_own<T, LPH>(p, t, p.k, p.k_row, p.k_head), v = load_own<T, LPH>(p, t, p.v, p.v_row, p.v_head);
+  const Counted<T, RAGGED> counted(t.skip);
   const int head0 = t.head * p.group;
   const Address qb = (Address)((const T *)p.q + head0 * p.q_head + t.d0), gb = (Address)((const T *)p.dout + head0 * p.dout_head + t.d0),
                 stb = (Address)(p.stats4 + head0);
@@ -675,7 +679,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backw
       read_ahead_fence();
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
-        const float s = group_sum<LPH>(dot_piece<T>(k, q[u])), d = group_sum<LPH>(dot_piece<T>(v, g[u]));
+        const float s = group_sum<LPH>(dot_piece<T>(k, counted.of(q[u]))), d = group_sum<LPH>(dot_piece<T>(v, counted.of(g[u])));
         const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - st[u][0]) * st[u][1] : 0.0f;
         const float ds = on[u] ? w * (d - st[u][2]) : 0.0f;
 #pragma unroll
@@ -872,16 +876,16 @@ static size_t stats4_bytes(const gcnx_attention *p) {
   return align_up((size_t)p->a->n_rows * p->n_heads * 16, 256);
 }
 
-template <typename T, int LPH, bool SHIFTS>
+template <typename T, int LPH, bool SHIFTS, bool RAGGED>
 static void launch_pass(int pass, const AttnArgs &p, dim3 grid, const AttnArgs &joined, dim3 joins, hipStream_t stream) {
   if (pass == kForward) {
-    hipLaunchKernelGGL((attention_forward_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
+    hipLaunchKernelGGL((attention_forward_kernel<T, LPH, SHIFTS, RAGGED>), grid, dim3(kBlock), 0, stream, p);
     if (p.part_floats) hipLaunchKernelGGL((attention_forward_join_kernel<T, LPH>), joins, dim3(kBlock), 0, stream, joined);
   } else if (pass == kBackwardRows) {
-    hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
+    hipLaunchKernelGGL((attention_backward_rows_kernel<T, LPH, SHIFTS, RAGGED>), grid, dim3(kBlock), 0, stream, p);
     if (p.part_floats) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, false>), joins, dim3(kBlock), 0, stream, joined);
   } else {
-    hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, SHIFTS>), grid, dim3(kBlock), 0, stream, p);
+    hipLaunchKernelGGL((attention_backward_columns_kernel<T, LPH, SHIFTS, RAGGED>), grid, dim3(kBlock), 0, stream, p);
     if (p.part_floats) hipLaunchKernelGGL((attention_backward_join_kernel<T, LPH, true>), joins, dim3(kBlock), 0, stream, joined);
   }
 }
@@ -915,8 +919,17 @@ static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   GCNX_REQUIRE(blocks < (1ll << 32) / kBlock && join_blocks < (1ll << 32) / kBlock, GCNX_ERR_UNSUPPORTED,
                "attention: %lld rows, %lld nonzeros and %d heads are too many for one launch", (long long)p.n_rows, (long long)p.nnz, heads);
   const dim3 joins((unsigned)join_blocks, (unsigned)join_tiles);
-  if (p.val || p.mask) launch_pass<T, LPH, true>(pass, p, grid, joined, joins, stream);
-  else launch_pass<T, LPH, false>(pass, p, grid, joined, joins, stream);
+  const bool shifts = p.val || p.mask;
+  if constexpr (LPH >= 2) {          // one lane's head is one piece, or shorter
+    if (p.dim % Piece<T>::N) {
+      if (shifts) launch_pass<T, LPH, true, true>(pass, p, grid, joined, joins, stream);
+      else launch_pass<T, LPH, false, true>(pass, p, grid, joined, joins, stream);
+      GCNX_CHECK_LAUNCH();
+      return GCNX_OK;
+    }
+  }
+  if (shifts) launch_pass<T, LPH, true, false>(pass, p, grid, joined, joins, stream);
+  else launch_pass<T, LPH, false, false>(pass, p, grid, joined, joins, stream);
   GCNX_CHECK_LAUNCH();
   return GCNX_OK;
 }

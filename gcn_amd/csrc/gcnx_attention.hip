@@ -1059,8 +1059,9 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
                GCNX_ERR_INVALID_ARG, "attention: the transpose does not belong to the matrix");
   GCNX_REQUIRE((at->n_rows == 0 || at->row_ptr) && (at->nnz == 0 || (at->col_idx && (!p->use_values || at->val))),
                GCNX_ERR_INVALID_ARG, "attention: null array in the transpose");
-  GCNX_REQUIRE(!p->edge_mask || at->nnz == 0 || t_mask_index, GCNX_ERR_INVALID_ARG,
-               "attention: the mask needs its index in the transpose");
+  // the nonzeros have one order in the matrix and another in the transpose
+  GCNX_REQUIRE(!p->edge_mask || at->nnz == 0 || p->mask_index || t_mask_index, GCNX_ERR_INVALID_ARG,
+               "attention: the mask needs its index in the matrix, or in the transpose, or in both");
   GCNX_REQUIRE(p->a->n_rows == 0 || (out && dout && stats && stride_ok(out_row) && stride_ok(out_head) && stride_ok(dout_row) && stride_ok(dout_head)),
                GCNX_ERR_INVALID_ARG, "attention: bad output or gradient of it");
   GCNX_REQUIRE(((uintptr_t)stats & 7) == 0 && ((uintptr_t)ws & 15) == 0, GCNX_ERR_INVALID_ARG, "attention: stats or workspace not aligned");

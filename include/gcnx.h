@@ -559,7 +559,8 @@ int gcnx_attention_forward(const gcnx_attention *p, const int32_t *chunk_row,
                            float *stats, void *ws, size_t ws_bytes, void *stream);
 /* Gradients of the above for the gradient `dout` of its output, from `out` and
  * `stats`; the probabilities are formed again.  `at` is the exact transpose of
- * p->a with its own chunk table, mask index and longest row.  dq [n_rows, n_heads,
+ * p->a with its own chunk table, mask index (nullable where p->mask_index is given: the
+ * mask is in the order of the transpose's nonzeros then) and longest row.  dq [n_rows, n_heads,
  * head_dim], dk, dv [n_cols, n_kv_heads, head_dim] (summed over the heads that share
  * them) are contiguous; dq alone or dk and dv alone may be asked for (the others
  * NULL).  The values and the mask get no gradient. */

@@ -174,3 +174,17 @@ def test_ops_refuse_cpu_tensors():
 
     with pytest.raises(RuntimeError):
         ops.attention(Pattern(), x.view(2, 1, 8), x.view(2, 1, 8), x.view(2, 1, 8))
+
+
+def test_a_mask_s_index_on_one_side_is_enough(lib):
+    """Either the matrix or its transpose may hold the nonzeros in the mask's order (the
+    call goes on to the next check, the workspace); both cannot."""
+    from gcn_amd import _lib
+    a, at = _csr(), _csr(5, 4, 6)
+
+    def bwd(midx, t_midx):
+        p = _attention(a, edge_mask=PTR, mask_index=midx)
+        return lib.gcnx_attention_backward(C.byref(p), PTR, C.byref(at), PTR, t_midx, 0, PTR, 32, 8, PTR, PTR, 32, 8, PTR, PTR, PTR, None, 0, None)
+
+    assert bwd(None, None) == _lib.ERR_INVALID_ARG
+    assert bwd(PTR, None) == bwd(None, PTR) == bwd(PTR, PTR) == _lib.ERR_WORKSPACE

@@ -93,3 +93,27 @@ def test_product(env):
             got = ops.spmm(t, torch.from_numpy(b).to(dev), mask=env["mask_dev"])
             # one rounding a product and a sum, at most 400 of them
             assert_within(got.cpu().numpy(), d @ b, 402 * U * (s @ np.abs(b)) + 1e-37, name)
+
+
+def test_mask_in_the_order_of_a_transpose_s_source(env):
+    """A matrix without an index of its own (mask in the order of its nonzeros) and its
+    transpose, whose index counts the same entries: forward and backward of both."""
+    torch, ops, dev = env["torch"], env["ops"], env["dev"]
+    b = env["a"].transpose(cache=False)
+    assert b.input_index is None
+    counts = (b.row_ptr[1:] - b.row_ptr[:-1]).cpu()
+    row = torch.repeat_interleave(torch.arange(b.n_rows), counts).numpy()
+    col = b.col_idx.cpu().numpy()
+    rng = np.random.RandomState(8)
+    mask = (rng.rand(b.nnz) < 0.7).astype(np.uint8)
+    t = b.transpose()
+    assert t.transpose() is b and t.input_nnz == b.nnz
+    for m, r, c in ((t, col, row), (b, row, col)):
+        make = lambda n: rng.standard_normal((n, 2, 8)).astype(np.float32)
+        q, k, v, g = make(m.n_rows), make(m.n_cols), make(m.n_cols), make(m.n_rows)
+        o = AttentionOracle(r, c, m.shape, *[x.astype(np.float64) for x in (q, k, v)], float(np.float32(8 ** -0.5)), None, mask).backward(g.astype(np.float64))
+        leaves = [torch.from_numpy(x).to(dev).requires_grad_(True) for x in (q, k, v)]
+        out = ops.attention_autograd(m, *leaves, mask=torch.from_numpy(mask).to(dev))
+        out.backward(torch.from_numpy(g).to(dev))
+        for what, got in zip(("out", "dq", "dk", "dv"), [out.detach()] + [x.grad for x in leaves]):
+            assert_within(got.cpu().numpy(), getattr(o, what), getattr(o, what + "_bound"), what)

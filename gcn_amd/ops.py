@@ -30,6 +30,13 @@ def _check_dense(t, name):
         raise ValueError("%s must be a row-major 2-D tensor" % name)
 
 
+def _written(*tensors):
+    """Counts a kernel's write to tensors that the caller holds, as torch counts its own
+    in-place operations: a backward pass that saved one of them refuses to run on what
+    is there now."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 # ------------------------------------------------------------------------ SpMM
 def spmm(a, b, out=None, alpha=1.0, beta=0.0, mask=None, mask_scale=1.0, relu=False, b2=None,
          dropout=None, sign_bits=None, dropout_rows=None):
@@ -68,6 +75,7 @@ def spmm(a, b, out=None, alpha=1.0, beta=0.0, mask=None, mask_scale=1.0, relu=Fa
         _check_dense(out, "out")
         if tuple(out.shape) != (a.n_rows, width):
             raise ValueError("out has shape %s, expected %s" % (tuple(out.shape), (a.n_rows, width)))
+        _written(out)
     midx = None
     if mask is not None:
         a.check_mask(mask)
@@ -90,6 +98,7 @@ def spmm(a, b, out=None, alpha=1.0, beta=0.0, mask=None, mask_scale=1.0, relu=Fa
                 sb.shape[1] * 32 < width or sb.stride(1) != 1 or sb.device != a.device or \
                 not spmm_supports_sign_bits(width):
             raise ValueError("sign_bits: int32 [n_rows, width / 32] on A's device, width % 32 == 0, no mask")
+        _written(sb)
         if dropout_rows is None:
             with torch.cuda.device(a.device):
                 need = lib.gcnx_spmm_workspace_bytes(a.struct_ref(), width)
@@ -162,6 +171,8 @@ def spmm_factored(a, d, w, gate_bits, gate_scale=1.0, trans_w=False, out=None, d
         out = torch.empty((a.n_rows, width), dtype=torch.float32, device=d.device)
     elif tuple(out.shape) != (a.n_rows, width) or out.stride(1) != 1:
         raise ValueError("out has shape %s, expected %s" % (tuple(out.shape), (a.n_rows, width)))
+    else:
+        _written(out)
     with torch.cuda.device(d.device):
         need = lib.gcnx_spmm_workspace_bytes(a.struct_ref(), width)
         ws = WORKSPACE.get(need, d.device)
@@ -268,6 +279,7 @@ def gemm(a, b, trans_a=False, trans_b=False, out=None, alpha=1.0, beta=0.0, relu
         _check_dense(out, "out")
         if tuple(out.shape) != (M, N):
             raise ValueError("out has shape %s, expected %s" % (tuple(out.shape), (M, N)))
+        _written(out)
     with torch.cuda.device(a.device):
         need = lib.gcnx_gemm_workspace_bytes(int(trans_a), int(trans_b), M, N, K)
         ws = WORKSPACE.get(need, a.device)
@@ -286,6 +298,7 @@ def gemm(a, b, trans_a=False, trans_b=False, out=None, alpha=1.0, beta=0.0, relu
                         or sign_bits.stride(1) != 1:
                     raise ValueError("sign_bits: int32 [M, N / 32], fused output dropout only (see "
                                      "gemm_supports_output_dropout), N % 32 == 0")
+                _written(sign_bits)
                 d = _lib.DropoutStruct(float(keep), int(seed) & (2 ** 64 - 1), int(offset), int(ld), int(col0))
                 _lib.check(lib.gcnx_gemm_relu_dropout_signs_f32(
                     int(trans_a), int(trans_b), M, N, K, _ptr(a), a.stride(0), _ptr(b), b.stride(0), _ptr(out),
@@ -383,6 +396,7 @@ def dropout_rows_philox(x, row_ids, keep, seed, offset, out=None):
         _check_dense(out, "out")
         if out.shape != x.shape:
             raise ValueError("out must have the shape of x")
+        _written(out)
     with torch.cuda.device(x.device):
         _lib.check(lib.gcnx_dropout_rows_philox_f32(x.shape[0], x.shape[1], _ptr(x), x.stride(0), _ptr(row_ids),
                                                     float(keep), int(seed) & (2 ** 64 - 1), int(offset),
@@ -404,6 +418,8 @@ def pack_sign_bits(x, rows=None, out=None):
         out = torch.empty((n, words), dtype=torch.int32, device=x.device)
     elif out.dtype != torch.int32 or tuple(out.shape) != (n, words) or out.stride(1) != 1:
         raise ValueError("out must be int32 [n, ceil(W/32)]")
+    else:
+        _written(out)
     with torch.cuda.device(x.device):
         _lib.check(lib.gcnx_pack_sign_bits_f32(n, _ptr(rows) if rows is not None else None, _ptr(x),
                                                x.stride(0), width, _ptr(out), out.stride(0), _stream()))
@@ -564,7 +580,8 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
     lib = _lib.load()
     p = _attention_struct(a, q, k, v, scale, use_values, mask)
     dev = q.device
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = _like(q)
         os = out.stride()
     else:
@@ -577,6 +594,8 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
         ws = _scratch(need, dev)
         _lib.check(lib.gcnx_attention_forward(C.byref(p), a.chunk_row.data_ptr(), out.data_ptr(), os[0], os[1], _at(stats), _at(ws),
                                               need, _stream_of(dev)))
+    if not fresh:
+        _written(out)
     return (out, stats) if want_stats else out
 
 
@@ -793,6 +812,8 @@ def masked_softmax_xent(logits, labels, mask, want_grad=True, mask_total=0.0, gr
             n, c, _ptr(logits), logits.stride(0), _ptr(labels), labels.stride(0), _ptr(mask),
             float(mask_total), _ptr(out), _ptr(grad), grad.stride(0) if grad is not None else 0,
             _ptr(ws), ws.numel(), _stream()))
+    if want_grad and grad_out is not None:
+        _written(grad_out)
     return out, grad
 
 
@@ -835,6 +856,7 @@ def counter_add(counter, inc=1):
         raise ValueError("counter must be a one-element int64 CUDA tensor")
     with torch.cuda.device(counter.device):
         _lib.check(lib.gcnx_counter_add_u64(_ptr(counter), int(inc), _stream()))
+    _written(counter)
     return counter
 
 
@@ -863,6 +885,8 @@ def bernoulli_mask(n, keep, seed, offset, device, out=None, step=None, step_stri
         else:
             _lib.check(lib.gcnx_bernoulli_mask_u8(int(n), float(keep), int(seed) & (2 ** 64 - 1),
                                                   int(offset), _ptr(mask), _stream()))
+    if out is not None:
+        _written(out)
     return mask
 
 
@@ -877,6 +901,7 @@ def dropout_dense(x, mask, scale, out=None):
     with torch.cuda.device(x.device):
         _lib.check(lib.gcnx_dropout_dense_f32(x.numel(), _ptr(x), _ptr(mask), float(scale),
                                               _ptr(out), _stream()))
+    _written(out)
     return out
 
 
@@ -893,6 +918,8 @@ def relu_dropout_bwd(y, dy, mask=None, scale=1.0, out=None):
     with torch.cuda.device(y.device):
         _lib.check(lib.gcnx_relu_dropout_bwd_f32(y.numel(), _ptr(y), _ptr(dy), _ptr(mask),
                                                  float(scale), _ptr(dx), _stream()))
+    if out is not None:
+        _written(out)
     return dx
 
 
@@ -908,6 +935,7 @@ def gather_rows(src, idx, out):
     with torch.cuda.device(src.device):
         _lib.check(lib.gcnx_gather_rows_f32(idx.numel(), _ptr(idx), _ptr(src), src.stride(0),
                                             src.shape[1], _ptr(out), out.stride(0), _stream()))
+    _written(out)
     return out
 
 
@@ -924,6 +952,7 @@ def scatter_rows(src, idx, out):
     with torch.cuda.device(src.device):
         _lib.check(lib.gcnx_scatter_rows_f32(idx.numel(), _ptr(idx), _ptr(src), src.stride(0),
                                              src.shape[1], _ptr(out), out.stride(0), _stream()))
+    _written(out)
     return out
 
 
@@ -980,6 +1009,7 @@ def dropout_philox(x, keep, seed, offset, out=None, mask_out=None):
         _lib.check(lib.gcnx_dropout_philox_f32(x.numel(), _ptr(x), float(keep),
                                                int(seed) & (2 ** 64 - 1), int(offset), _ptr(out),
                                                _ptr(mask_out), _stream()))
+    _written(out) if mask_out is None else _written(out, mask_out)
     return out
 
 
@@ -994,6 +1024,8 @@ def relu_dropout_bwd_philox(y, dy, keep, seed, offset, out=None):
         _lib.check(lib.gcnx_relu_dropout_bwd_philox_f32(y.numel(), _ptr(y), _ptr(dy), float(keep),
                                                         int(seed) & (2 ** 64 - 1), int(offset),
                                                         _ptr(dx), _stream()))
+    if out is not None:
+        _written(out)
     return dx
 
 
@@ -1031,6 +1063,7 @@ def adam_step(w, grad, m, v, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, weight_dec
             _lib.check(lib.gcnx_adam_step_f32(w.numel(), _ptr(w), _ptr(grad), _ptr(m), _ptr(v),
                                               float(lr), float(beta1), float(beta2), float(eps),
                                               float(weight_decay), int(t), _stream()))
+    _written(w, m, v)
     return w
 
 
@@ -1144,6 +1177,7 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
         need = _lib.ADAMW_WORKSPACE_BYTES if t_ptr else 0
         ws = _scratch(need, dev)
         _lib.check(lib.gcnx_adamw_step(C.byref(p), count, table.ctypes.data, _at(ws), need, _stream_of(dev)))
+    _written(*[p for p, n in zip(params, sizes) if n])
     return params
 
 

@@ -618,7 +618,7 @@ def attention_bwd(a, q, k, v, out, stats, d_out, scale=None, use_values=False, m
         return None, None, None
     if a._t is None and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("attention_bwd under a stream capture: build a.transpose() before it")
-    at = a.transpose()
+    at = a.transpose() if use_values or a._t is None else a._t        # its values may be old ones where they are not read
     longest = at.max_row_nnz()
     dq = _like(q) if need_q else None
     dk = dv = None
@@ -640,14 +640,14 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, a, scale, use_values, mask):
         out, stats = attention(a, q, k, v, scale, use_values, mask, want_stats=True)
-        ctx.save_for_backward(q, k, v, out, stats, mask)
+        ctx.save_for_backward(q, k, v, out, stats, mask, a.val if use_values else None)
         ctx.how = (a, scale, use_values)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, out, stats, mask = ctx.saved_tensors
+        q, k, v, out, stats, mask, _values = ctx.saved_tensors       # the values: refused here if written since
         a, scale, use_values = ctx.how
         if d_out.stride(2) != 1 and d_out.shape[2] > 1:
             d_out = d_out.contiguous()

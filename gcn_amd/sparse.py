@@ -82,7 +82,8 @@ class Csr(object):
         self.input_index = input_index
         self.input_nnz = self.nnz if input_index is None or input_nnz is None else int(input_nnz)
         self.device = row_ptr.device
-        self._t = None
+        self._t = None           # the cached transpose, whether it was built from this matrix, what its values go by
+        self._t_built, self._t_seen = False, None
         self._max_row = None
         self.gather_keep = None
         self._struct = _lib.CsrStruct(self.n_rows, self.n_cols, self.nnz,
@@ -280,34 +281,55 @@ class Csr(object):
         return cls.from_coo(m.row, m.col, m.data, m.shape, device)
 
     # --------------------------------------------------------------- transpose
-    def transpose(self, cache=True):
-        """Exact transpose (cached).  Its ``input_index`` still refers to the
-        tuple this matrix was built from, so a dropout mask drawn for the
-        forward product can be reused by the backward one.  ``cache=False``: a
-        fresh matrix that neither is remembered by this one nor remembers it, and
-        carries no ``input_index`` (set-up of derived matrices)."""
-        if cache and self._t is not None:
-            return self._t
+    def _transposed(self, val=None, want_perm=True):
+        """The arrays of the exact transpose: ``(row_ptr, col_idx, val, perm)``."""
         lib = _lib.load()
         dev = self.device
-        t_row_ptr = torch.empty(self.n_cols + 1, dtype=torch.int64, device=dev)
-        t_col_idx = torch.empty(self.nnz, dtype=torch.int32, device=dev)
-        t_val = torch.empty(self.nnz, dtype=torch.float32, device=dev)
-        t_perm = torch.empty(self.nnz, dtype=torch.int64, device=dev) if cache else None
+        row_ptr = torch.empty(self.n_cols + 1, dtype=torch.int64, device=dev)
+        col_idx = torch.empty(self.nnz, dtype=torch.int32, device=dev)
+        if val is None:
+            val = torch.empty(self.nnz, dtype=torch.float32, device=dev)
+        perm = torch.empty(self.nnz, dtype=torch.int64, device=dev) if want_perm else None
         with torch.cuda.device(dev):
             need = lib.gcnx_csr_transpose_workspace_bytes(self.n_rows, self.n_cols, self.nnz)
             ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
-            _lib.check(lib.gcnx_csr_transpose(self.struct_ref(), _ptr(t_row_ptr), _ptr(t_col_idx),
-                                              _ptr(t_val), _ptr(t_perm), _ptr(ws), ws.numel(),
-                                              _stream()))
-        del ws
+            _lib.check(lib.gcnx_csr_transpose(self.struct_ref(), _ptr(row_ptr), _ptr(col_idx), _ptr(val), _ptr(perm),
+                                              _ptr(ws), ws.numel(), _stream()))
+        return row_ptr, col_idx, val, perm
+
+    def transpose(self, cache=True):
+        """Exact transpose (cached).  Its ``input_index`` still refers to the
+        tuple this matrix was built from, so a dropout mask drawn for the
+        forward product can be reused by the backward one.  Values written in
+        place since are taken over at the next call (not under a stream capture); a
+        transpose whose own values were written stays as it is and a new one is
+        made.  ``cache=False``: a fresh matrix that neither is remembered by this
+        one nor remembers it, and carries no ``input_index`` (set-up of derived
+        matrices)."""
         if not cache:
-            return Csr(self.n_cols, self.n_rows, t_row_ptr, t_col_idx, t_val, None)
-        idx = self.input_index[t_perm] if self.input_index is not None else t_perm
-        t = Csr(self.n_cols, self.n_rows, t_row_ptr, t_col_idx, t_val, idx, self.input_nnz)
-        t._t = self
-        self._t = t
-        return t
+            row_ptr, col_idx, val, _ = self._transposed(want_perm=False)
+            return Csr(self.n_cols, self.n_rows, row_ptr, col_idx, val, None)
+        if self._t is not None and self._t_seen == self._versions():
+            return self._t
+        if self._t is not None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the matrix's values were written since its transpose was built: "
+                               "call transpose() before the stream capture")
+        if self._t is not None and self._t_built and self._t_seen[1] == self._versions()[1]:
+            self._transposed(self._t.val, want_perm=False)
+            torch.autograd.graph.increment_version(self._t.val)
+        else:
+            row_ptr, col_idx, val, perm = self._transposed()
+            idx = self.input_index[perm] if self.input_index is not None else perm
+            self._t = Csr(self.n_cols, self.n_rows, row_ptr, col_idx, val, idx, self.input_nnz)
+            self._t._t = self
+            self._t_built = True
+        self._t_seen = self._versions()
+        self._t._t_seen = self._t._versions()
+        return self._t
+
+    def _versions(self):
+        """How often torch or a kernel of ops wrote this matrix's and its transpose's values."""
+        return tuple(None if m.val.is_inference() else m.val._version for m in (self, self._t))
 
     # ------------------------------------------------------------------ export
     def to_scipy(self):

@@ -1094,6 +1094,25 @@ class AdamWState(object):
         self._table = np.zeros(len(self.sizes), dtype=[("w", "u8"), ("grad", "u8"), ("n", "i8"), ("state", "i8"), ("decay", "f8")])
         self._table["state"] = self.offsets
 
+    def _parts(self, i):
+        """Tensor i's part of every buffer (8-bit codes as bytes)."""
+        at, end = self.offsets[i], self.offsets[i] - (-self.sizes[i] // _lib.ADAMW_BLOCK) * _lib.ADAMW_BLOCK
+        codes = [t.view(torch.uint8) if self.bits == 8 else t for t in (self.exp_avg, self.exp_avg_sq)]
+        scales = [self.exp_avg_scale, self.exp_avg_sq_scale] if self.bits == 8 else []
+        return [t[at:end] for t in codes] + [t[at // _lib.ADAMW_BLOCK:end // _lib.ADAMW_BLOCK] for t in scales]
+
+    def reset(self, i):
+        """Zeroes the moments of tensor i."""
+        for part, value in zip(self._parts(i), (0, 0, 1, 1)):
+            part.fill_(value)
+
+    def take(self, i, other, j):
+        """Copies the moments of tensor j of another state of the same ``bits`` to tensor i."""
+        if other.bits != self.bits or other.sizes[j] != self.sizes[i]:
+            raise ValueError("states or tensors differ")
+        for to, part in zip(self._parts(i), other._parts(j)):
+            to.copy_(part)
+
     def moments(self, i):
         """``(m, v)`` of tensor i as flat float32 tensors."""
         at, n = self.offsets[i], self.sizes[i]

@@ -19,6 +19,7 @@ import contextlib
 import os
 import sys
 import warnings
+import weakref
 
 import numpy as np
 import torch
@@ -523,16 +524,23 @@ class AdamOptimizer(object):
     def minimize(self, loss):
         return _OptOp(self, loss)
 
+    def _count(self):
+        """Advances the step count, on the device and (outside a capture) on the host."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        if self._step_dev is None:
+            if capturing:      # set by the recording, the count would be set back by every replay
+                raise RuntimeError("%s: run a step before the stream capture" % type(self).__name__)
+            self._step_dev = ops.device_counter(device(), self.step)
+        if not capturing:
+            self.step += 1
+        ops.counter_add(self._step_dev, 1)
+
     def apply(self, variables, grads, decay=None):
         """One update of every variable; ``decay`` maps a variable to the
         coefficient of its weight-decay term (gradient added in the kernel).  The step count lives in device memory
         and is advanced by a kernel, so that the launches can be recorded in a
         HIP graph and replayed."""
-        if self._step_dev is None:
-            self._step_dev = ops.device_counter(device(), self.step)
-        if not torch.cuda.is_current_stream_capturing():
-            self.step += 1
-        ops.counter_add(self._step_dev, 1)
+        self._count()
         decay = decay or {}
         for v, g in zip(variables, grads):
             wd = decay.get(v, 0.0)
@@ -545,37 +553,95 @@ class AdamOptimizer(object):
                               self._step_dev, self.beta1, self.beta2, self.epsilon, weight_decay=wd)
 
 
+class _AdamWGroup(object):
+    """Variables that an AdamWOptimizer met together, and their moments."""
+
+    def __init__(self, variables, state):
+        self.refs = [weakref.ref(v) for v in variables]
+        self.tensors = [v.tensor for v in variables]
+        self.state = state
+
+    def without_the_gone(self):
+        """The group of the variables that still exist: itself if all do, None if none does."""
+        kept = [(i, r()) for i, r in enumerate(self.refs) if r() is not None]
+        if len(kept) == len(self.refs) or not kept:
+            return self if kept else None
+        tensors = [self.tensors[i] for i, _ in kept]
+        state = ops.adamw_state(tensors, self.state.bits, self.state.seed)
+        for to, (i, _) in enumerate(kept):
+            state.take(to, self.state, i)
+        group = _AdamWGroup([v for _, v in kept], state)
+        group.tensors = tensors                 # those the moments belong to
+        return group
+
+
 class AdamWOptimizer(AdamOptimizer):
     """Adam with decoupled weight decay over all variables in one launch
     (:func:`gcn_amd.ops.adamw_step`), its moments in 32 or in 8 bits
     (``state_bits``; for weights of a graph's size, the first layer of a featureless
-    model).  Weight-decay terms of the loss stay what they are, a gradient."""
+    model).  Weight-decay terms of the loss stay what they are, a gradient.  A
+    variable that is loaded or initialised again starts with new moments, the others
+    keep theirs; variables that come later are a launch of their own."""
 
     def __init__(self, learning_rate=0.001, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, state_bits=32, seed=0):
         super(AdamWOptimizer, self).__init__(learning_rate, beta1, beta2, epsilon)
         self.weight_decay, self.state_bits, self.seed = weight_decay, state_bits, seed
-        self._state = None     # (the variables' tensors, their moments)
+        self._groups = []
+        self._made = 0
+        self._place = {}       # id of a variable -> its group and place there
+
+    def _find(self, v):
+        group, i = self._place.get(id(v), (None, 0))
+        return (group, i) if group is not None and group.refs[i]() is v else (None, 0)
+
+    def _admit(self, variables):
+        """Moments for every variable: kept, zeroed where its storage is new, or made."""
+        later = []
+        for v in variables:
+            group, i = self._find(v)
+            if group is not None and group.tensors[i] is v.tensor:
+                continue
+            if torch.cuda.is_current_stream_capturing():
+                # zeroed by the recording, moments would be zeroed by every replay
+                raise RuntimeError("AdamWOptimizer: variable %s is new, or was initialised or loaded: run a step before the capture" % v.name)
+            if group is not None:
+                group.state.reset(i)
+                group.tensors[i] = v.tensor
+            else:
+                later.append(v)
+        if later:
+            self._groups = [g for g in [g.without_the_gone() for g in self._groups] if g is not None]
+            # a key of its own for every group: elements are counted from 0 in each
+            group = _AdamWGroup(later, ops.adamw_state([v.tensor for v in later], self.state_bits, self.seed + self._made))
+            self._made += 1
+            self._groups.append(group)
+            self._place = {id(r()): (g, i) for g in self._groups for i, r in enumerate(g.refs) if r() is not None}
+
+    def moments(self, variable):
+        """``(m, v)`` of a variable as flat float32 tensors."""
+        group, i = self._find(variable)
+        if group is None:
+            raise ValueError("no step has been taken with variable %s" % variable.name)
+        return group.state.moments(i)
 
     def apply(self, variables, grads, decay=None):
         decay = decay or {}
-        tensors = [v.tensor for v in variables]
-        if self._state is None or len(self._state[0]) != len(tensors) or any(a is not b for a, b in zip(self._state[0], tensors)):
-            # new storage (a variable initialised or loaded): new moments, as Variable.load says
-            self._state = (tensors, ops.adamw_state(tensors, self.state_bits, self.seed))
-        if self._step_dev is None:
-            self._step_dev = ops.device_counter(device(), self.step)
-        if not torch.cuda.is_current_stream_capturing():
-            self.step += 1
-        ops.counter_add(self._step_dev, 1)
-        full = []
+        variables = list(variables)
+        if len(set(map(id, variables))) != len(variables):
+            raise ValueError("a variable is there twice")
+        self._admit(variables)
+        self._count()
+        full = {id(g): [None] * len(g.tensors) for g in self._groups}
         with torch.no_grad():
             for v, g in zip(variables, grads):
                 coef = decay.get(v, 0.0)
                 if coef:
                     g = v.tensor * coef if g is None else g.add(v.tensor, alpha=coef)
-                full.append(g.contiguous() if g is not None else None)
-            ops.adamw_step(tensors, full, self._state[1], self.learning_rate, self._step_dev, self.beta1, self.beta2, self.epsilon,
-                           self.weight_decay)
+                group, i = self._find(v)
+                full[id(group)][i] = g.contiguous() if g is not None else None
+            for group in self._groups:
+                ops.adamw_step(group.tensors, full[id(group)], group.state, self.learning_rate, self._step_dev, self.beta1, self.beta2,
+                               self.epsilon, self.weight_decay)
 
 
 class _Saver(object):

@@ -301,8 +301,7 @@ class Variable(Node):
         self.name = (scope + "/" if scope else "") + (name or "Variable") + ":0"
         self._initial = initial
         self.tensor = None
-        self.adam_m = None
-        self.adam_v = None
+        self._adam = None
         arr = initial() if callable(initial) else np.asarray(initial)
         self._init_value = np.ascontiguousarray(arr, dtype=np.float32)
         self.static_shape = self._init_value.shape
@@ -311,8 +310,33 @@ class Variable(Node):
     def initialize(self):
         _VAR_EPOCH[0] += 1
         self.tensor = torch.from_numpy(self._init_value.copy()).to(device()).requires_grad_(True)
-        self.adam_m = torch.zeros_like(self.tensor, requires_grad=False)
-        self.adam_v = torch.zeros_like(self.tensor, requires_grad=False)
+        self._adam = None
+
+    def _adam_moments(self):
+        """AdamOptimizer's two moments, made when they are first asked for: other
+        optimizers have moments of their own."""
+        if self._adam is None and self.tensor is not None:
+            if torch.cuda.is_current_stream_capturing():
+                # zeroed by the recording, they would be zeroed by every replay
+                raise RuntimeError("variable %s has no Adam moments yet: run a step before the stream capture" % self.name)
+            self._adam = [torch.zeros_like(self.tensor, requires_grad=False) for _ in range(2)]
+        return self._adam or [None, None]
+
+    @property
+    def adam_m(self):
+        return self._adam_moments()[0]
+
+    @adam_m.setter
+    def adam_m(self, value):
+        self._adam = [value, self._adam_moments()[1]]
+
+    @property
+    def adam_v(self):
+        return self._adam_moments()[1]
+
+    @adam_v.setter
+    def adam_v(self, value):
+        self._adam = [self._adam_moments()[0], value]
 
     def load(self, value, sess=None):
         """Overwrite the value (resets the Adam moments)."""

@@ -190,3 +190,36 @@ def test_first_step_under_a_capture_is_refused(env):
         torch.cuda.synchronize()
         assert torch.equal(a.tensor, twin.tensor)
         assert all(torch.equal(x, y) for x, y in zip(opt.moments(a), other.moments(twin)))
+
+
+def test_no_memory_for_another_optimizer_s_moments(env):
+    """A step with 8-bit state holds the weights and 2 + 1/32 bytes an element."""
+    torch, tf = env["torch"], env["tf"]
+    tf.reset_default_graph()
+    gc.collect()
+    n = 1 << 22
+    small, = _variables(env, (256,))
+    tf.train.AdamWOptimizer(0.01, state_bits=8).apply([small], _grads(env, [small], 0))      # loads the code
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    big, = _variables(env, (n,))
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before <= 4 * n + 4096
+    opt = tf.train.AdamWOptimizer(0.01, state_bits=8)
+    opt.apply([big], [torch.ones(n, device=env["dev"])])
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before <= 4 * n + 2 * n + n // 32 + 8192
+    # the plain optimizer's are there when it asks, and start over with the variable
+    adam = tf.train.AdamOptimizer(0.01)
+    adam.apply([small], _grads(env, [small], 1))
+    assert small.adam_m.any() and small.adam_v.any() and small.adam_m is small.adam_m
+    small.load(np.zeros(256, np.float32))
+    assert small.adam_m.shape == (256,) and not small.adam_m.any() and not small.adam_v.any()
+    # recorded as a first step they would be zeroed by every replay
+    fresh, = _variables(env, (16,))
+    g = _grads(env, [fresh], 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the stream capture"):
+        with torch.cuda.graph(graph):
+            adam.apply([fresh], g)

@@ -732,9 +732,10 @@ def norm_residual(x, z=None, gate=None, post_weight=None, res_scale=None, pre_we
 
 
 def norm_residual_bwd(x, dy, dh, stats, z=None, gate=None, post_weight=None, res_scale=None, pre_weight=None, kind="rms",
-                      eps=1e-6):
+                      eps=1e-6, need=(True,) * 6):
     """``(dx, dz, dgate, dpost, dres, dpre)`` of :func:`norm_residual` for the gradients
-    ``dy`` and ``dh`` of its outputs (None: zero); None where there is no such operand.
+    ``dy`` and ``dh`` of its outputs (None: zero); None where there is no such operand
+    and where ``need`` (one flag a gradient) is False.
     The row gradients have the type of ``x``, those of the weights are float32, summed
     over the rows in a fixed order."""
     lib = _lib.load()
@@ -747,24 +748,24 @@ def norm_residual_bwd(x, dy, dh, stats, z=None, gate=None, post_weight=None, res
     dev = x.device
     if stats.dtype != torch.float32 or stats.shape != (n, 4) or not stats.is_contiguous() or stats.device != dev:
         raise ValueError("stats must be what norm_residual(..., want_stats=True) returned")
-    dx = _like(x)
-    dz = _like(x) if z is not None else None
-    dgate = _like(x) if gate is not None else None
+    dx = _like(x) if need[0] else None
+    dz = _like(x) if z is not None and need[1] else None
+    dgate = _like(x) if gate is not None and need[2] else None
     made = [None, None, None]
-    wanted = [i for i, w in enumerate((post_weight, res_scale, pre_weight)) if w is not None]
+    wanted = [i for i, w in enumerate((post_weight, res_scale, pre_weight)) if w is not None and need[3 + i]]
     summed = [i for i in wanted if n and (i < 2 or dh is not None)]
     if wanted:
         # one buffer for the (small) gradients of the weights; sums over nothing are zero
         buf = (torch.empty if len(summed) == len(wanted) else torch.zeros)((len(wanted), dim), dtype=torch.float32, device=dev)
         for row, i in zip(buf.unbind(0), wanted):
             made[i] = row
-    if n:
+    if n and (dx is not None or dz is not None or dgate is not None or summed):
         with _on(dev):
-            need = lib.gcnx_norm_residual_backward_workspace_bytes(C.byref(p)) if summed else 0
-            ws = _scratch(need, dev)
+            room = lib.gcnx_norm_residual_backward_workspace_bytes(C.byref(p)) if summed else 0
+            ws = _scratch(room, dev)
             _lib.check(lib.gcnx_norm_residual_backward(
-                C.byref(p), _at(dy), dy_ld, _at(dh), dh_ld, stats.data_ptr(), dx.data_ptr(), _at(dz), _at(dgate), _at(made[0]),
-                _at(made[1]), _at(made[2]) if dh is not None else None, _at(ws), need, _stream_of(dev)))
+                C.byref(p), _at(dy), dy_ld, _at(dh), dh_ld, stats.data_ptr(), _at(dx), _at(dz), _at(dgate), _at(made[0]),
+                _at(made[1]), _at(made[2]) if dh is not None else None, _at(ws), room, _stream_of(dev)))
     return (dx, dz, dgate) + tuple(made)
 
 
@@ -782,7 +783,8 @@ class _NormResidualFn(torch.autograd.Function):
     def backward(ctx, dy, dh):
         x, z, gate, post_weight, res_scale, pre_weight, stats = ctx.saved_tensors
         rows = lambda t: t if t is None or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-        return norm_residual_bwd(x, rows(dy), rows(dh), stats, z, gate, post_weight, res_scale, pre_weight, *ctx.how) + (None, None)
+        return norm_residual_bwd(x, rows(dy), rows(dh), stats, z, gate, post_weight, res_scale, pre_weight, *ctx.how,
+                                 need=ctx.needs_input_grad[:6]) + (None, None)
 
 
 def norm_residual_autograd(x, z=None, gate=None, post_weight=None, res_scale=None, pre_weight=None, kind="rms", eps=1e-6):

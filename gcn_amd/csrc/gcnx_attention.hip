@@ -1065,8 +1065,10 @@ extern "C" int gcnx_attention_backward(const gcnx_attention *p, const int32_t *c
   GCNX_REQUIRE(p->a->n_rows == 0 || (out && dout && stats && stride_ok(out_row) && stride_ok(out_head) && stride_ok(dout_row) && stride_ok(dout_head)),
                GCNX_ERR_INVALID_ARG, "attention: bad output or gradient of it");
   GCNX_REQUIRE(((uintptr_t)stats & 7) == 0 && ((uintptr_t)ws & 15) == 0, GCNX_ERR_INVALID_ARG, "attention: stats or workspace not aligned");
-  GCNX_REQUIRE((dk == nullptr) == (dv == nullptr) && (dq || dk || (p->a->n_rows == 0 && p->a->n_cols == 0)),
+  // gradients of no rows, or of no columns, are empty tensors, whose address may be null
+  GCNX_REQUIRE((dk == nullptr) == (dv == nullptr) && (dq || dk || p->a->n_rows == 0 || p->a->n_cols == 0),
                GCNX_ERR_INVALID_ARG, "attention: dq, or dk and dv, or all three");
+  if (!dq && !dk) return GCNX_OK;
   const size_t need = gcnx_attention_backward_workspace_bytes(p, t_max_row_nnz);
   GCNX_REQUIRE(need == 0 || (ws && ws_bytes >= need), GCNX_ERR_WORKSPACE,
                "attention: workspace of %zu bytes needed, %zu given", need, ws_bytes);

@@ -188,3 +188,20 @@ def test_a_mask_s_index_on_one_side_is_enough(lib):
 
     assert bwd(None, None) == _lib.ERR_INVALID_ARG
     assert bwd(PTR, None) == bwd(None, PTR) == bwd(PTR, PTR) == _lib.ERR_WORKSPACE
+
+
+def test_gradients_of_no_rows_and_of_no_columns(lib):
+    """Empty gradients have no address: nothing to do is no error."""
+    from gcn_amd import _lib
+
+    def bwd(rows, cols, **kw):
+        a, at = _csr(rows, cols, 0), _csr(cols, rows, 0)
+        f = dict(out=PTR, stats=PTR, dout=PTR, dq=None, dk=None, dv=None)
+        f.update(kw)
+        return lib.gcnx_attention_backward(C.byref(_attention(a)), PTR, C.byref(at), PTR, None, 0, f["out"], 32, 8, f["stats"], f["dout"],
+                                           32, 8, f["dq"], f["dk"], f["dv"], PTR, 1 << 40, None)
+
+    for shape in ((0, 0), (0, 5), (4, 0)):
+        assert bwd(*shape) == _lib.OK, shape
+    assert bwd(4, 5) == _lib.ERR_INVALID_ARG                       # there are some: asked for none of them
+    assert bwd(4, 0, dk=PTR) == _lib.ERR_INVALID_ARG               # dk without dv

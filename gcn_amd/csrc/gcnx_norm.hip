@@ -51,7 +51,7 @@ template <typename T, int TPR>
 __device__ __forceinline__ Place place(int dim) {
   constexpr int W = TPR ? TPR : 1, N = Piece<T>::N;
   Place a;
-  a.slot = threadIdx.x / W;
+  a.slot = TPR > kWave ? 0 : threadIdx.x / W;       // one row a workgroup there: the row is a scalar
   a.d0 = (threadIdx.x % W) * N;
   a.live = a.d0 < dim;
   a.skip = 0;
@@ -83,10 +83,16 @@ __device__ __forceinline__ f32x2 row_sum(f32x2 v, float *sh, int &turn) {
     turn ^= 1;
     if ((threadIdx.x & (kWave - 1)) == 0) half[threadIdx.x / kWave] = v;
     __syncthreads();
-    f32x2 t = half[0];
+    if constexpr (kWaves == 16) {
+      // 1024 lanes have 128 registers each: 32 of them for the 16 pairs were spilled
+      const f32x2 t = half[threadIdx.x % kWaves];
+      return f32x2{group_sum<kWaves>(t[0]), group_sum<kWaves>(t[1])};
+    } else {
+      f32x2 t = half[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) t += half[w];
-    return t;
+      for (int w = 1; w < kWaves; ++w) t += half[w];
+      return t;
+    }
   }
 }
 
@@ -352,11 +358,20 @@ static int threads_per_row(int dtype, int dim) {
 
 static int64_t rows_per_block(int tpr) { return tpr > kWave ? 1 : kBlock / (tpr ? tpr : 1); }
 
-// Workgroups that stay: `deep` a CU, as many as its registers hold at once (2^20 x 256
-// bf16, 8 and 4 a CU -> 3 and 2: forward 600 -> 542 us, backward 990 -> 827: the
-// backward pass writes a partial sum of the columns a workgroup).
+// Workgroups that stay: `deep` times 256 lanes a CU, in whole workgroups and at least
+// one, fewer than the registers would hold (6 and 3 in 16 bits).  The backward pass
+// writes a partial sum of the columns a workgroup; a CU with half a workgroup more than
+// its neighbours ends last, and one without any idles.
+// us forward / backward at 1, 2, 3, 4, 8 (rows x elements):
+//   2^22 x 16, fp32     371/439  290/460  284/453  285/482  292/499   bf16  218/236  151/248  158/248  159/267  162/261
+//   2^18 x 500, fp32    865/970  565/964  603/1005 608/1018 625/1025  bf16  421/422  290/466  291/490  298/514  309/500
+//   2^20 x 256, fp32   1508/1740 1081/1719 1094/1689 1176/1785 1178/1795 bf16 763/818 531/839  546/890  582/1027 608/1094
+//   2^17 x 1024, fp32   692/800  532/963  536/882  572/981  569/1038  bf16  438/516  291/444  285/456  281/487  283/492
+// (1024 lanes a row, 2^15 x 4096 fp32: 64 x deep workgroups 523/1117, one a CU 494/800;
+// 512 lanes, 2^15 x 4096 bf16: one and a half a CU 284/470, one 251/429.)
 static int64_t norm_blocks(int64_t n, int tpr, int64_t deep) {
-  const int64_t every = ceil_div(n, rows_per_block(tpr)), most = 256 * deep * kBlock / (tpr > kWave ? tpr : kBlock);
+  const int64_t every = ceil_div(n, rows_per_block(tpr)), a_cu = deep * kBlock / (tpr > kWave ? tpr : kBlock);
+  const int64_t most = 256 * (a_cu > 1 ? a_cu : 1);
   return every < most ? every : most;
 }
 constexpr int64_t kForwardDeep = 3, kBackwardDeep = 2;

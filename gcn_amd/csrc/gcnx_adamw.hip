@@ -16,7 +16,10 @@
 // the same state on any launch geometry.  An element that is not finite keeps a NaN
 // code and leaves its block's scale to the others.  Arithmetic is fp32, one rounding
 // an operation (no contraction), so that the codes are those of the formulas above
-// computed operation by operation.
+// computed operation by operation.  The one exception is the division of the step,
+// which is the hardware's reciprocal (1 ulp) and a product: two more roundings of a
+// term that is about lr, below the rounding of the weight that it changes, for a
+// quarter of the division's instructions.
 //
 // Bound by memory: 28 bytes an element with fp32 weights, gradients and state, 14 with
 // fp32 weights, bf16 gradients and 8-bit state (scales are 1/32 byte each).  A
@@ -376,9 +379,12 @@ extern "C" int gcnx_adamw_step(const gcnx_adamw *q, int64_t n_tensors, const gcn
     p.root = (float)(1.0 / sqrt(1.0 - pow(q->beta2, (double)q->t)));
   }
   // Tiles a wavefront has in flight: 4 where they fill the machine (8 wavefronts a
-  // SIMD), else 1, so that more of it takes part.  A step that moves more than the
-  // 256 MiB Infinity Cache holds streams past the caches: nothing of it is there when
-  // the next step comes (0.36 G fp32 elements: 1.69 ms against 1.88).
+  // SIMD), else 1, so that more of it takes part.  A step over more than the 256 MiB
+  // that the Infinity Cache holds (weights, gradients, state) streams past the caches:
+  // nothing of it is there when the next step comes.  us streamed / not, fp32 with
+  // 32-bit state: 362 M elements 1760 / 1890, 48 M 229 / 258, 24 M 118 / 129; still
+  // 86 / 82 at 17 M (272 MB), and 75 / 69 at 14 M (224 MB), which does not stream; bf16
+  // gradients and 8-bit state: 362 M 875 / 1010, 48 M 130 / 137, 24 M (192 MB) 70 / 68.
   const int64_t bytes = total * ((q->w_dtype == GCNX_F32 ? 4 : 2) + (q->g_dtype == GCNX_F32 ? 4 : 2) + (eight ? 2 : 8));
   const Size size = total / (4 * kTile) < 8 * 1024 ? kSmall : bytes <= (256ll << 20) ? kDeep : kStream;
   const int64_t per_block = (int64_t)kTile * kWavesPerBlock * (size == kSmall ? 1 : 4);

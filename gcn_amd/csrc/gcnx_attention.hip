@@ -15,8 +15,11 @@
 // transpose: every sum has one owner and a fixed order, so there are no atomics and
 // results are the same bits run to run.
 //
-// What bounds it: 4 (7 or 10 backward) flops an element gathered leave the matrix units
-// nothing to do; k and v of every edge are read through the caches.  2^19 nodes, 8.9 M
+// What bounds it: k and v of every edge are read through the caches, and where every
+// query head has its own keys 4 (7 or 10 backward) flops an element gathered leave the
+// matrix units nothing to do.  (Heads that share keys gather less and compute the same:
+// there the vector ALU bounds the forward and the row pass, 70 to 75 % busy at 8 on 2;
+// their scores are products of a kind that the matrix units could take.)  2^19 nodes, 8.9 M
 // edges, 8 heads of 32, bf16: forward 1.03 ms, row pass 1.15, column pass 1.25 for 9.1,
 // 9.1 and 10.3 GB gathered; a quarter of it hits L2, the rest comes at 6.4 to 6.8 TB/s,
 // what the fabric behind the L2s gives.  Operands within the caches: 2^16 nodes, forward
@@ -847,6 +850,9 @@ static int64_t part_floats(int pass, int dtype, int heads, int kv_heads, int dim
 // The forward pass with its join, us, at 64 / 128 / 256 / 512 (heads of 4 x 16, 8 on
 // 2 x 64, 8 x 32, 8 x 32): 0.1 M edges 24 / 26 / 28 / 39, 0.9 M 177 / 181 / 220 / 256,
 // 1 M 108 / 109 / 109 / 138, 8.5 M 1130 / 1096 / 1046 / 1057.
+// Forward / backward at 128, 256, 512: 17.1 M (8 x 32 bf16) 2341/5315, 2299/5250,
+// 2249/5158; (8 x 16 fp32) 2187/5137, 2184/5122, 2145/5033; 34.5 M (4 x 16 fp32)
+// 2487/5935, 2444/5872, 2291/5554; 8.5 M (8 x 32 fp32) 2441/5195, 2401/5117, 2421/5228.
 // Where rows average over 1024 pieces their joins are what takes long, and pieces get
 // longer: 2^20 edges of 3 rows 133 / 111 / 95 / 115.
 static int segment_of(int64_t nnz, int64_t n_rows) {

@@ -13,6 +13,7 @@ All functions raise on CPU tensors -- there is no fallback path.
 """
 import contextlib
 import ctypes as C
+import operator
 
 import numpy as np
 import torch
@@ -1094,7 +1095,7 @@ class AdamWState(object):
             self.exp_avg_scale, self.exp_avg_sq_scale = [torch.ones_like(zeros(total // _lib.ADAMW_BLOCK, torch.float32))
                                                          for _ in range(2)]
         self._table = np.zeros(len(self.sizes), dtype=[("w", "u8"), ("grad", "u8"), ("n", "i8"), ("state", "i8"), ("decay", "f8")])
-        self._table["state"] = self.offsets
+        self._table["state"], self._table["n"] = self.offsets, self.sizes
 
     def _parts(self, i):
         """Tensor i's part of every buffer (8-bit codes as bytes)."""
@@ -1143,6 +1144,27 @@ def adamw_state(params, bits=32, seed=0):
     return AdamWState(params, bits, seed)
 
 
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _uniform(tensors, dtype, index, sizes):
+    """Whether all are contiguous tensors of one type on GPU ``index``, of these sizes
+    (attribute by attribute: half the time of a loop over the tensors)."""
+    return set(map(_dtype_of, tensors)) == {dtype} and set(map(torch.Tensor.get_device, tensors)) == {index} and \
+        list(map(torch.Tensor.numel, tensors)) == sizes and all(map(torch.Tensor.is_contiguous, tensors))
+
+
+def _overlap(addresses, sizes, itemsize):
+    """Whether one of the tensors, taken in this order, begins before the end of an earlier one."""
+    end = 0
+    for at, n in zip(addresses, sizes):
+        if n:
+            if at < end:
+                return True
+            end = at + n * itemsize
+    return False
+
+
 def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01):
     """One in-place AdamW update of every tensor of ``params`` in one launch (one per 64
     tensors): ``m = beta1 m + (1 - beta1) g``, ``v = beta2 v + (1 - beta2) g^2``,
@@ -1158,47 +1180,39 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
     params, grads = list(params), list(grads)
     if len(params) != count or len(grads) != count:
         raise ValueError("%d params and %d grads for a state of %d tensors" % (len(params), len(grads), count))
-    dtype, dev, g_dtype = state.dtype, state.device, None
-    w_ptr, g_ptr, sizes = [], [], []
-    for p, g, n in zip(params, grads, state.sizes):
-        if p.dtype != dtype or p.device != dev or p.numel() != n or not p.is_contiguous():
-            raise ValueError("params must be the contiguous tensors the state was made for")
-        if g is None:
-            w_ptr.append(p.data_ptr())
-            g_ptr.append(0)
-            sizes.append(0)
-            continue
-        if g_dtype is None:
-            g_dtype = g.dtype
-            if g_dtype not in _DTYPES:
-                raise TypeError("grads must be float32, bfloat16 or float16, got %s" % (g_dtype,))
-        if g.dtype != g_dtype or g.device != dev or g.numel() != n or not g.is_contiguous():
-            raise ValueError("grads must be contiguous, of one dtype, on the params' device and of their sizes")
-        w_ptr.append(p.data_ptr())
-        g_ptr.append(g.data_ptr())
-        sizes.append(n)
-    size = dtype.itemsize
-    live = sorted([(w, w + n * size) for w, n in zip(w_ptr, sizes) if n])
-    if not live:
+    dtype, dev, table, sizes = state.dtype, state.device, state._table, state.sizes
+
+    if not _uniform(params, dtype, dev.index, sizes):
+        raise ValueError("params must be the contiguous tensors the state was made for")
+    live, wanted, decay = params, [i for i, g in enumerate(grads) if g is not None], weight_decay
+    if len(wanted) < count:
+        live, grads, sizes = [[x[i] for i in wanted] for x in (params, grads, sizes)]
+        table, decay = table[wanted], np.broadcast_to(np.asarray(decay, dtype=np.float64), count)[wanted]
+    if not any(sizes):
         return params
-    for a, b in zip(live, live[1:]):
-        if b[0] < a[1]:
-            raise ValueError("params share memory")
+    g_dtype = grads[0].dtype
+    if g_dtype not in _DTYPES:
+        raise TypeError("grads must be float32, bfloat16 or float16, got %s" % (g_dtype,))
+    if not _uniform(grads, g_dtype, dev.index, sizes):
+        raise ValueError("grads must be contiguous, of one dtype, on the params' device and of their sizes")
+    w_ptr, g_ptr = list(map(torch.Tensor.data_ptr, live)), list(map(torch.Tensor.data_ptr, grads))
+    if _overlap(w_ptr, sizes, dtype.itemsize) and _overlap(*zip(*sorted(zip(w_ptr, sizes))), dtype.itemsize):
+        raise ValueError("params share memory")
     if isinstance(t, torch.Tensor):
         if t.device != dev or t.dtype != torch.int64 or t.numel() != 1:
             raise ValueError("t must be an int or a one-element int64 tensor on the params' device")
         t_ptr, t_host = t.data_ptr(), 0
     else:
         t_ptr, t_host = None, int(t)
-    table = state._table.copy()
-    table["w"], table["grad"], table["n"], table["decay"] = w_ptr, g_ptr, sizes, weight_decay
+    table = table.copy()
+    table["w"], table["grad"], table["decay"] = w_ptr, g_ptr, decay
     p = _lib.AdamWStruct(_DTYPES[dtype], _DTYPES[g_dtype], state.bits, state.exp_avg.data_ptr(), state.exp_avg_sq.data_ptr(),
                          _at(state.exp_avg_scale), _at(state.exp_avg_sq_scale), lr, beta1, beta2, eps, t_host, t_ptr, state.seed)
     with _on(dev):
         need = _lib.ADAMW_WORKSPACE_BYTES if t_ptr else 0
         ws = _scratch(need, dev)
-        _lib.check(lib.gcnx_adamw_step(C.byref(p), count, table.ctypes.data, _at(ws), need, _stream_of(dev)))
-    _written(*[p for p, n in zip(params, sizes) if n])
+        _lib.check(lib.gcnx_adamw_step(C.byref(p), len(table), table.ctypes.data, _at(ws), need, _stream_of(dev)))
+    _written(*live)
     return params
 
 

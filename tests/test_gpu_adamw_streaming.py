@@ -27,7 +27,7 @@ def _part(ops, state, at, n):
     part.__dict__.update(state.__dict__)
     part.sizes, part.offsets = [n], [at]
     part._table = state._table[:1].copy()
-    part._table["state"] = at
+    part._table["state"], part._table["n"] = at, n
     return part
 
 

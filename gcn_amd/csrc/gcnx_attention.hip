@@ -54,6 +54,41 @@ __device__ __forceinline__ float dot_piece(const typename Piece<T>::raw &a, cons
   return d;
 }
 
+// A piece without the elements that another lane counts, or that there are none of.
+template <typename T, int LPH>
+__device__ __forceinline__ typename Piece<T>::raw counted(typename Piece<T>::raw x, int skip, int dim) {
+#pragma unroll
+  for (int i = 0; i < Piece<T>::N; ++i)
+    if (LPH ? i < skip : i >= dim) x[i] = (T)0.0f;
+  return x;
+}
+
+// The sums over a head of own * x and of own2 * x2.  RAGGED: a head that is no multiple
+// of a piece.  The lane's own operand is zero where it does not count, which leaves
+// the other side's element out unless that is not finite: 0 * inf.  A NaN of that
+// origin cannot be told from another by the sum, so the products of a wavefront that
+// meets one are formed again with zeros on both sides.  (Zeros on both sides for
+// every edge: backward of 4.2 M edges at 8 x 20 bf16 1140 us against 1040, at 4 x 5
+// 1303 against 1066.)
+template <typename T, int LPH, bool RAGGED>
+__device__ __forceinline__ float head_dot(const typename Piece<T>::raw &own, const typename Piece<T>::raw &x, int skip, int dim) {
+  float s = group_sum<LPH>(dot_piece<T>(own, x));
+  if constexpr (RAGGED)
+    if (__any(s != s)) s = group_sum<LPH>(dot_piece<T>(own, counted<T, LPH>(x, skip, dim)));
+  return s;
+}
+template <typename T, int LPH, bool RAGGED>
+__device__ __forceinline__ f32x2 head_dots(const typename Piece<T>::raw &own, const typename Piece<T>::raw &x, const typename Piece<T>::raw &own2,
+                                           const typename Piece<T>::raw &x2, int skip, int dim) {
+  float s = group_sum<LPH>(dot_piece<T>(own, x)), d = group_sum<LPH>(dot_piece<T>(own2, x2));
+  if constexpr (RAGGED)
+    if (__any(s != s || d != d)) {
+      s = group_sum<LPH>(dot_piece<T>(own, counted<T, LPH>(x, skip, dim)));
+      d = group_sum<LPH>(dot_piece<T>(own2, counted<T, LPH>(x2, skip, dim)));
+    }
+  return f32x2{s, d};
+}
+
 __device__ __forceinline__ bool is_lowest(float x) { return x == -__builtin_inff(); }
 
 // Edges in flight per lane: more cost registers, so wavefronts, and idle slots at the
@@ -64,10 +99,9 @@ constexpr int kBackwardEdges = 1;
 
 // Wavefronts a SIMD that the registers have to leave room for: 8 (64 registers) where
 // nothing is spilled for it.  (Column pass at 2^19 nodes: 1284 us against 1525 with
-// the 5 that the compiler chooses.)  The backward passes of ragged heads hold four
-// words more.
-template <int LPH, bool SHIFTS, bool RAGGED = false>
-constexpr int kWaves = SHIFTS && LPH == 0 ? 5 : SHIFTS || LPH == 0 || LPH >= 32 ? 6 : RAGGED ? 7 : 8;
+// the 5 that the compiler chooses.)
+template <int LPH, bool SHIFTS>
+constexpr int kWaves = SHIFTS && LPH == 0 ? 5 : SHIFTS || LPH == 0 || LPH >= 32 ? 6 : 8;
 
 struct AttnArgs {
   // pattern walked by this pass (the matrix, or its transpose)
@@ -312,7 +346,6 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forwa
   if (!find_task<T, LPH>(p, p.heads, t)) return;
   const int kv = t.head / p.group;
   const raw q = load_own<T, LPH>(p, t, p.q, p.q_row, p.q_head);
-  const Counted<T, RAGGED> counted(t.skip);
   float acc[N] = {}, m = -__builtin_inff(), l = 0.0f;
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (t.count) {
@@ -334,7 +367,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_forwa
       float top = m;
 #pragma unroll
       for (int u = 0; u < kForwardEdges; ++u) {
-        const float d = group_sum<LPH>(dot_piece<T>(q, counted.of(k[u])));
+        const float d = head_dot<T, LPH, RAGGED>(q, k[u], t.skip, p.dim);
         s[u] = on[u] ? fmaf(d, p.scale, s[u]) : -__builtin_inff();
         top = fmaxf(top, s[u]);
       }
@@ -535,7 +568,7 @@ __device__ __forceinline__ typename Piece<T>::raw load_row(const AttnArgs &p, co
 }
 
 template <typename T, int LPH, bool SHIFTS, bool RAGGED>
-__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attention_backward_rows_kernel(AttnArgs p) {
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_rows_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   __shared__ float sh[2 * N + 1][kWave];
@@ -544,7 +577,6 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attenti
   const int kv = t.head / p.group;
   float acc[N] = {}, low[N] = {}, m, r, d0, rest = 0.0f;
   const raw q = load_own<T, LPH>(p, t, p.q, p.q_row, p.q_head), g = load_row<T, LPH>(p, t, m, r, d0);
-  const Counted<T, RAGGED> counted(t.skip);
   const Address kb = (Address)((const T *)p.k + kv * p.k_head + t.d0), vb = (Address)((const T *)p.v + kv * p.v_head + t.d0);
   if (!kCorrected<T> && !p.o0) t.count = 0;        // delta alone is asked for
   if (t.count) {
@@ -565,7 +597,8 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attenti
       read_ahead_fence();
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
-        const float s = group_sum<LPH>(dot_piece<T>(q, counted.of(k[u]))), d = group_sum<LPH>(dot_piece<T>(g, counted.of(v[u])));
+        const f32x2 sd = head_dots<T, LPH, RAGGED>(q, k[u], g, v[u], t.skip, p.dim);
+        const float s = sd[0], d = sd[1];
         const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - m) * r : 0.0f;
         const float ds = on[u] ? w * (d - d0) : 0.0f;
         rest += ds;
@@ -627,7 +660,7 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attenti
 // the key heads; the edges of the column are walked once per query head that
 // shares the key head, as count * group items.
 template <typename T, int LPH, bool SHIFTS, bool RAGGED>
-__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attention_backward_columns_kernel(AttnArgs p) {
+__global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS>)) void attention_backward_columns_kernel(AttnArgs p) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::raw raw;
   __shared__ float sh[2 * N][kWave];
@@ -635,7 +668,6 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attenti
   if (!find_task<T, LPH>(p, p.kv_heads, t)) return;
   float dk[N] = {}, dv[N] = {};
   const raw k = load_own<T, LPH>(p, t, p.k, p.k_row, p.k_head), v = load_own<T, LPH>(p, t, p.v, p.v_row, p.v_head);
-  const Counted<T, RAGGED> counted(t.skip);
   const int head0 = t.head * p.group;
   const Address qb = (Address)((const T *)p.q + head0 * p.q_head + t.d0), gb = (Address)((const T *)p.dout + head0 * p.dout_head + t.d0),
                 stb = (Address)(p.stats4 + head0);
@@ -682,7 +714,8 @@ __global__ __launch_bounds__(kBlock, (kWaves<LPH, SHIFTS, RAGGED>)) void attenti
       read_ahead_fence();
 #pragma unroll
       for (int u = 0; u < kBackwardEdges; ++u) {
-        const float s = group_sum<LPH>(dot_piece<T>(k, counted.of(q[u]))), d = group_sum<LPH>(dot_piece<T>(v, counted.of(g[u])));
+        const f32x2 sd = head_dots<T, LPH, RAGGED>(k, q[u], v, g[u], t.skip, p.dim);
+        const float s = sd[0], d = sd[1];
         const float w = on[u] ? exp_of(fmaf(s, p.scale, shift[u]) - st[u][0]) * st[u][1] : 0.0f;
         const float ds = on[u] ? w * (d - st[u][2]) : 0.0f;
 #pragma unroll
@@ -925,17 +958,18 @@ static int launch_lanes(int pass, AttnArgs p, hipStream_t stream) {
   GCNX_REQUIRE(blocks < (1ll << 32) / kBlock && join_blocks < (1ll << 32) / kBlock, GCNX_ERR_UNSUPPORTED,
                "attention: %lld rows, %lld nonzeros and %d heads are too many for one launch", (long long)p.n_rows, (long long)p.nnz, heads);
   const dim3 joins((unsigned)join_blocks, (unsigned)join_tiles);
-  const bool shifts = p.val || p.mask;
-  if constexpr (LPH >= 2) {          // one lane's head is one piece, or shorter
-    if (p.dim % Piece<T>::N) {
+  // one lane's head is a piece, or shorter; several lanes' may be a multiple of one
+  const bool shifts = p.val || p.mask, ragged = LPH == 0 || p.dim % Piece<T>::N != 0;
+  if constexpr (LPH != 1)
+    if (ragged) {
       if (shifts) launch_pass<T, LPH, true, true>(pass, p, grid, joined, joins, stream);
       else launch_pass<T, LPH, false, true>(pass, p, grid, joined, joins, stream);
-      GCNX_CHECK_LAUNCH();
-      return GCNX_OK;
     }
-  }
-  if (shifts) launch_pass<T, LPH, true, false>(pass, p, grid, joined, joins, stream);
-  else launch_pass<T, LPH, false, false>(pass, p, grid, joined, joins, stream);
+  if constexpr (LPH != 0)
+    if (!ragged) {
+      if (shifts) launch_pass<T, LPH, true, false>(pass, p, grid, joined, joins, stream);
+      else launch_pass<T, LPH, false, false>(pass, p, grid, joined, joins, stream);
+    }
   GCNX_CHECK_LAUNCH();
   return GCNX_OK;
 }

@@ -40,7 +40,7 @@ __device__ const f32x4 g_zeros[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
 __device__ __forceinline__ Address at_or_zeros(Address a, bool on) { return on ? a : (Address)&g_zeros[0]; }
 
 // One piece.  Rows need only their elements' alignment: global loads of 16 bytes
-// take any address.  NARROW: `dim` < a piece, the rest is zero.
+// take any address.  NARROW: `dim` < a piece, the rest repeats the last element.
 template <typename T, bool NARROW>
 __device__ __forceinline__ typename Piece<T>::raw load_piece(Address a, int dim) {
   typedef typename Piece<T>::raw raw;
@@ -50,10 +50,7 @@ __device__ __forceinline__ typename Piece<T>::raw load_piece(Address a, int dim)
   } else {
     raw x;
 #pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i) {
-      const T e = load_at<T>(a + sizeof(T) * (i < dim ? i : dim - 1));
-      x[i] = i < dim ? e : (T)0.0f;
-    }
+    for (int i = 0; i < Piece<T>::N; ++i) x[i] = load_at<T>(a + sizeof(T) * (i < dim ? i : dim - 1));
     return x;
   }
 }
@@ -71,28 +68,6 @@ __device__ __forceinline__ void store_piece(T *p, int dim, const float (&v)[Piec
       if (i < dim) p[i] = (T)v[i];
   }
 }
-
-// What a lane counts of a gathered piece in a product with its own: the elements that
-// another lane counts (RAGGED: heads that are no multiple of a piece) become zero on
-// this side too, not only in the lane's own operand, for 0 * inf is NaN.
-template <typename T, bool RAGGED>
-struct Counted {
-  typedef uint32_t words __attribute__((ext_vector_type(4)));
-  words keep;
-  __device__ __forceinline__ explicit Counted(int skip) {
-    if constexpr (RAGGED) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) keep[i] = i < skip ? 0u : ~0u;
-        else keep[i] = (2 * i < skip ? 0u : 0xffffu) | (2 * i + 1 < skip ? 0u : 0xffff0000u);
-      }
-    }
-  }
-  __device__ __forceinline__ typename Piece<T>::raw of(const typename Piece<T>::raw &x) const {
-    if constexpr (RAGGED) return __builtin_bit_cast(typename Piece<T>::raw, __builtin_bit_cast(words, x) & keep);
-    else return x;
-  }
-};
 
 // Sum over groups of G neighbouring lanes, the result in every lane of the group.
 // Steps 1..8 are moves on the vector ALU: quad permutes, then the mirrors of 8 and

@@ -13,7 +13,6 @@ All functions raise on CPU tensors -- there is no fallback path.
 """
 import contextlib
 import ctypes as C
-import operator
 
 import numpy as np
 import torch
@@ -538,7 +537,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(device):
     """Makes ``device`` current for the launches of a ``with`` block."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _stream_of(device):
@@ -1144,14 +1143,15 @@ def adamw_state(params, bits=32, seed=0):
     return AdamWState(params, bits, seed)
 
 
-_dtype_of = operator.attrgetter("dtype")
+_numel_of, _index_of, _dense, _address_of = torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 
 
 def _uniform(tensors, dtype, index, sizes):
     """Whether all are contiguous tensors of one type on GPU ``index``, of these sizes
     (attribute by attribute: half the time of a loop over the tensors)."""
-    return set(map(_dtype_of, tensors)) == {dtype} and set(map(torch.Tensor.get_device, tensors)) == {index} and \
-        list(map(torch.Tensor.numel, tensors)) == sizes and all(map(torch.Tensor.is_contiguous, tensors))
+    n = len(sizes)
+    return [t.dtype for t in tensors].count(dtype) == n and list(map(_index_of, tensors)).count(index) == n and \
+        list(map(_numel_of, tensors)) == sizes and all(map(_dense, tensors))
 
 
 def _overlap(addresses, sizes, itemsize):
@@ -1195,7 +1195,7 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
         raise TypeError("grads must be float32, bfloat16 or float16, got %s" % (g_dtype,))
     if not _uniform(grads, g_dtype, dev.index, sizes):
         raise ValueError("grads must be contiguous, of one dtype, on the params' device and of their sizes")
-    w_ptr, g_ptr = list(map(torch.Tensor.data_ptr, live)), list(map(torch.Tensor.data_ptr, grads))
+    w_ptr, g_ptr = list(map(_address_of, live)), list(map(_address_of, grads))
     if _overlap(w_ptr, sizes, dtype.itemsize) and _overlap(*zip(*sorted(zip(w_ptr, sizes))), dtype.itemsize):
         raise ValueError("params share memory")
     if isinstance(t, torch.Tensor):

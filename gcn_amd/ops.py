@@ -567,10 +567,10 @@ def attention(a, q, k, v, scale=None, use_values=False, mask=None, out=None, wan
     with the matrix values as logit shifts only if ``use_values``; query head ``h``
     reads key head ``h' = h // (heads / kv_heads)``.  ``q`` [n_rows, heads, head_dim],
     ``k`` and ``v`` [n_cols, kv_heads, head_dim], float32, bfloat16 or float16, any
-    strides between head vectors; ``scale`` defaults to ``head_dim ** -0.5``.
-    ``mask`` (uint8, in the order of the tuple ``A`` was built from) takes the
-    edges with 0 out of the softmax, as a value of -inf does; a row with no edge
-    left gives zeros.  ``out`` (default: a new tensor) must not share memory with
+    strides below 2^30 between head vectors; ``scale`` defaults to ``head_dim ** -0.5``.
+    ``mask`` (uint8, in the order of the tuple ``a`` was built from, ``a.input_nnz``
+    bytes) takes the edges with 0 out of the softmax, as a value of -inf does; a row
+    with no edge left gives zeros.  ``out`` (default: a new tensor) must not share memory with
     ``q``, ``k`` or ``v``.  With ``want_stats`` returns ``(out, stats)``, what
     :func:`attention_bwd` needs.  The longest row of ``a`` is looked up at its first
     use (a host synchronisation; skipped under a stream capture, where it is taken as

@@ -525,9 +525,9 @@ int gcnx_gemm_dropout_at_rows_f32(int64_t M, int64_t N, int64_t K, const float *
  * -inf: its rows of k and v are not read for it.  A row without an edge that takes
  * part gives zeros.  Operands: dtype elements, q [n_rows, n_heads, head_dim],
  * k and v [n_cols, n_kv_heads, head_dim], rows of head_dim (1..256) contiguous
- * elements, other strides in elements (0 allowed, not negative).  Logits, softmax
- * and sums are fp32, results are rounded once.  Sums have a fixed order: results
- * are bitwise reproducible.
+ * elements, other strides in elements (0 allowed, not negative, below 2^30); up to
+ * 65535 heads.  Logits, softmax and sums are fp32, results are rounded once.  Sums
+ * have a fixed order: results are bitwise reproducible.
  * Rows longer than 64 .. 512 edges (by the edges and rows of the matrix) are shared by the
  * wavefronts of a workgroup, very long ones (8 times that, or where max_row_nnz, the
  * most edges of a row, is 0 = unknown) cut into pieces joined by a second launch:

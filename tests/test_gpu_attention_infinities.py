@@ -3,7 +3,7 @@ probability of zero, and what that edge's other elements hold changes nothing.""
 import numpy as np
 import pytest
 
-from attention_oracle import U, assert_within
+from attention_oracle import U
 
 pytestmark = pytest.mark.gpu
 

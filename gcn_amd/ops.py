@@ -640,7 +640,7 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, a, scale, use_values, mask):
         out, stats = attention(a, q, k, v, scale, use_values, mask, want_stats=True)
-        ctx.save_for_backward(q, k, v, out, stats, mask, a.val if use_values else None)
+        ctx.save_for_backward(q, k, v, out, stats, mask, a.val if use_values and not a.val.is_inference() else None)
         ctx.how = (a, scale, use_values)
         return out
 

@@ -180,3 +180,17 @@ def test_values_written_before_a_capture(env):
         torch.cuda.synchronize()
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+def test_matrix_made_in_inference_mode(env):
+    """Its values have no version counter and cannot be saved: they are trusted."""
+    torch, ops, dev = env["torch"], env["ops"], env["dev"]
+    from gcn_amd.sparse import Csr
+    rng = np.random.RandomState(2)
+    with torch.inference_mode():
+        a = Csr.from_coo(rng.randint(0, 20, 100), rng.randint(0, 20, 100), rng.standard_normal(100), (20, 20), dev)
+        q = torch.randn(20, 1, 8, device=dev)
+        ops.attention(a, q, q, q, use_values=True, out=torch.empty_like(q))
+    leaves = _leaves(env)
+    ops.attention_autograd(a, *leaves, use_values=True).sum().backward()
+    assert all(torch.isfinite(t.grad).all() for t in leaves) and a.transpose() is a.transpose()

@@ -584,9 +584,13 @@ class _AdamWGroup(object):
         self.refs = [weakref.ref(v) for v in variables]
         self.tensors = [v.tensor for v in variables]
         self.state = state
+        self.recorded = False
 
     def without_the_gone(self):
-        """The group of the variables that still exist: itself if all do, None if none does."""
+        """The group of the variables that still exist: itself if all do, None if none
+        does.  One that a recorded launch writes stays as it is."""
+        if self.recorded:
+            return self
         kept = [(i, r()) for i, r in enumerate(self.refs) if r() is not None]
         if len(kept) == len(self.refs) or not kept:
             return self if kept else None
@@ -644,8 +648,8 @@ class AdamWOptimizer(AdamOptimizer):
     def moments(self, variable):
         """``(m, v)`` of a variable as flat float32 tensors."""
         group, i = self._find(variable)
-        if group is None:
-            raise ValueError("no step has been taken with variable %s" % variable.name)
+        if group is None or group.tensors[i] is not variable.tensor:
+            raise ValueError("no step has been taken with variable %s as it is" % variable.name)
         return group.state.moments(i)
 
     def apply(self, variables, grads, decay=None):
@@ -656,6 +660,7 @@ class AdamWOptimizer(AdamOptimizer):
         self._admit(variables)
         self._count()
         full = {id(g): [None] * len(g.tensors) for g in self._groups}
+        capturing = torch.cuda.is_current_stream_capturing()
         with torch.no_grad():
             for v, g in zip(variables, grads):
                 coef = decay.get(v, 0.0)
@@ -663,6 +668,7 @@ class AdamWOptimizer(AdamOptimizer):
                     g = v.tensor * coef if g is None else g.add(v.tensor, alpha=coef)
                 group, i = self._find(v)
                 full[id(group)][i] = g.contiguous() if g is not None else None
+                group.recorded = group.recorded or capturing
             for group in self._groups:
                 ops.adamw_step(group.tensors, full[id(group)], group.state, self.learning_rate, self._step_dev, self.beta1, self.beta2,
                                self.epsilon, self.weight_decay)

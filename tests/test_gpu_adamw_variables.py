@@ -176,6 +176,8 @@ def test_first_step_under_a_capture_is_refused(env):
     with pytest.raises(RuntimeError, match="run a step before the capture"):
         record()
     opt.apply([a], g)
+    with pytest.raises(ValueError):
+        opt.moments(_variables(env, (3,))[0])
     twin, = _variables(env, (1000,))
     twin.load(a.numpy())
     m, v = _moments(opt, a)
@@ -223,3 +225,38 @@ def test_no_memory_for_another_optimizer_s_moments(env):
     with pytest.raises(RuntimeError, match="before the stream capture"):
         with torch.cuda.graph(graph):
             adam.apply([fresh], g)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_recorded_moments_stay_where_they_are(env, bits):
+    """One variable of a recorded step is gone and another has come: the recording goes
+    on over the memory that it knows, bit for bit as without all that."""
+    torch, tf = env["torch"], env["tf"]
+    tf.reset_default_graph()
+    pairs = []
+    for _ in range(2):
+        both = _variables(env, (1000,), (700,))
+        opt = tf.train.AdamWOptimizer(0.01, state_bits=bits)
+        opt.apply(both, _grads(env, both, 0))
+        pairs.append((opt, both))
+    (opt, both), (other, twins) = pairs
+    grads = _grads(env, both, 1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.apply(both, grads)
+    a, state = both[0], opt._groups[0].state
+    for turn in range(5):
+        graph.replay()
+        other.apply(twins, grads)
+        if turn == 1:
+            del pairs, both
+            tf.reset_default_graph()
+            gc.collect()
+            late = _variables(env, (900,))
+            opt.apply(late, _grads(env, late, 3))
+            opt._step_dev -= 1
+            assert opt._groups[0].state is state and len(opt._groups) == 2
+        torch.cuda.synchronize()
+        assert torch.equal(a.tensor, twins[0].tensor)
+        assert all(torch.equal(x, y) for x, y in zip(opt.moments(a), other.moments(twins[0])))

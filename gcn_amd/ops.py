@@ -1184,8 +1184,9 @@ def adamw_step(params, grads, state, lr, t, beta1=0.9, beta2=0.999, eps=1e-8, we
 
     if not _uniform(params, dtype, dev.index, sizes):
         raise ValueError("params must be the contiguous tensors the state was made for")
-    live, wanted, decay = params, [i for i, g in enumerate(grads) if g is not None], weight_decay
-    if len(wanted) < count:
+    live, decay = params, weight_decay
+    if type(None) in map(type, grads):
+        wanted = [i for i, g in enumerate(grads) if g is not None]
         live, grads, sizes = [[x[i] for i in wanted] for x in (params, grads, sizes)]
         table, decay = table[wanted], np.broadcast_to(np.asarray(decay, dtype=np.float64), count)[wanted]
     if not any(sizes):
